@@ -17,6 +17,7 @@ static inline size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 static inline size_t elem_size(int dtype) { return dtype == FDMLA_F32 ? 4 : 2; }
 static inline bool dtype_ok(int dtype) { return dtype == FDMLA_F32 || dtype == FDMLA_BF16; }
 
+void note_kernel(const char *family) { t_last_kernel = family; }
 bool tensor_kernels_allowed() { return g_backend.load() != FDMLA_BACKEND_PORTABLE; }
 
 static int run_forward(const FwdProblem &p, int dtype, cudaStream_t stream) {
@@ -141,8 +142,8 @@ int fdmla_set_single_cta(int on) { tensor_prefer_single_cta(on != 0); return FDM
 const char *fdmla_last_kernel(void) { return t_last_kernel; }
 int fdmla_device_error_flag(int reset) {
     const int fwd = tensor_error_flag(reset), bwd = bwd_tensor_error_flag(reset), gemm = gemm_error_flag(reset),
-              xch = exchange_error_flag(reset);
-    return fwd ? fwd : (bwd ? bwd : (gemm ? gemm : xch));
+              xch = exchange_error_flag(reset), cache = cache_error_flag(reset);
+    return fwd ? fwd : (bwd ? bwd : (gemm ? gemm : (xch ? xch : cache)));
 }
 
 size_t fdmla_exchange_bytes(int world, long long rows, int d_v) { return exchange_bytes(world, rows, d_v); }

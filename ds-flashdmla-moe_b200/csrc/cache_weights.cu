@@ -1,0 +1,448 @@
+// A latent cache that may not grow: the attention weight every cached row has received, and the eviction of the rows that
+// received least ("consume K_lat/V_lat from the KV-cache", README.md:15 of the reference, is all it says about the cache).
+//
+// Beside the pool [num_pages, page_size, d] stand weights [num_pages, page_size] fp32 and positions [num_pages, page_size]
+// int32, addressed through the same page table:
+//   accumulate:  weights[row of key t] += sum over the query rows r that see t of exp(scale q_r . k_t - m_r) / l_r
+//                with the m, l that the attention of the same step returned
+//   evict:       of a sequence with more than `keep` rows the newest stay (position >= next - recent), then the heaviest,
+//                ties: the lower row.  Survivors in front of row `keep` do not move, the others fill the evicted rows'
+//                places, both in ascending order, so as few rows as possible are copied and no copy reads what another
+//                writes.  The attention does not depend on the order of the rows (their rotary part holds the position).
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <math_constants.h>
+#include <stdint.h>
+
+#include "common.cuh"
+#include "ptx.cuh"
+
+namespace fdmla {
+namespace cw {
+
+constexpr int ERR_PAGE = 4;                      // the code the attention kernels use for a bad page id or length
+__device__ int g_cache_error = 0;
+
+struct Pages {
+    const int32_t *table;                        // [B, max_pages]
+    const int32_t *seqlens;                      // [B]
+    int page_size, max_pages, num_pages;
+    __device__ __forceinline__ int length(int b) const {
+        const int n = seqlens[b], cap = max_pages * page_size;
+        if (n < 0 || n > cap) { g_cache_error = ERR_PAGE; return n < 0 ? 0 : cap; }
+        return n;
+    }
+    // physical row of logical row t of sequence b, or -1
+    __device__ __forceinline__ long long row(int b, int t) const {
+        const int lp = t / page_size, pg = table[(size_t)b * max_pages + lp];
+        if (pg < 0 || pg >= num_pages) { g_cache_error = ERR_PAGE; return -1; }
+        return (long long)pg * page_size + (t - lp * page_size);
+    }
+};
+
+struct AccProblem {
+    const void *Q, *pool;                        // [B, R, d] with R = H Sq rows (row r is query r mod Sq), [num_pages, page_size, d]
+    const float *m, *l;                          // [B, R]
+    float *weights;                              // [num_pages, page_size]
+    Pages pg;
+    int B, R, Sq, d, causal;
+    float scale_log2;                            // softmax scale times log2(e)
+};
+
+// ---- accumulate on CUDA cores: any type and width ---------------------------------------------------------------------------
+// Block: 32 keys of one sequence (a lane owns a key, its row in shared memory) x all query rows, four rows per warp at a time.
+constexpr int ACC_WARPS = 8, ACC_ROWS = 4;
+
+template <typename T>
+__global__ void __launch_bounds__(ACC_WARPS * 32) accumulate_simt_kernel(const AccProblem p) {
+    extern __shared__ float s_k[];               // [32][d + 1], then [ACC_WARPS][32]
+    const int b = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int n = p.pg.length(b), t0 = blockIdx.x * 32, t = t0 + lane, ld = p.d + 1;
+    if (t0 >= n) return;
+    for (int j = warp; j < 32; j += ACC_WARPS) {
+        const long long row = t0 + j < n ? p.pg.row(b, t0 + j) : -1;
+        const T *src = static_cast<const T *>(p.pool) + row * p.d;
+        for (int i = lane; i < p.d; i += 32) s_k[j * ld + i] = row >= 0 ? to_f32(src[i]) : 0.f;
+    }
+    __syncthreads();
+    float got = 0.f;
+    for (int r0 = warp * ACC_ROWS; r0 < p.R; r0 += ACC_WARPS * ACC_ROWS) {
+        float s[ACC_ROWS] = {};
+        const T *q[ACC_ROWS];
+#pragma unroll
+        for (int j = 0; j < ACC_ROWS; ++j)
+            q[j] = static_cast<const T *>(p.Q) + ((size_t)b * p.R + (r0 + j < p.R ? r0 + j : r0)) * p.d;
+        for (int i = 0; i < p.d; ++i) {
+            const float k = s_k[lane * ld + i];
+#pragma unroll
+            for (int j = 0; j < ACC_ROWS; ++j) s[j] = fmaf(to_f32(q[j][i]), k, s[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < ACC_ROWS; ++j) {
+            const int r = r0 + j;
+            if (r >= p.R) break;
+            const float l = p.l[(size_t)b * p.R + r], m = p.m[(size_t)b * p.R + r];
+            const int last = p.causal ? r % p.Sq + n - p.Sq : n - 1;
+            if (l <= 0.f || t > last) continue;            // a row without a visible key gives nothing
+            got += exp2f(fmaf(s[j], p.scale_log2, -m * 1.4426950408889634f)) / l;
+        }
+    }
+    __syncthreads();
+    s_k[warp * 32 + lane] = got;
+    __syncthreads();
+    if (warp == 0 && t < n) {
+        float sum = 0.f;
+        for (int w = 0; w < ACC_WARPS; ++w) sum += s_k[w * 32 + lane];
+        const long long row = p.pg.row(b, t);
+        if (row >= 0) atomicAdd(p.weights + row, sum);     // one addition per key; atomic in case sequences share a page
+    }
+}
+
+// ---- new rows: no weight yet, positions counted on ---------------------------------------------------------------------------
+__global__ void __launch_bounds__(128) stamp_kernel(float *__restrict__ weights, int32_t *__restrict__ positions,
+                                                    const int32_t *__restrict__ table, const int32_t *__restrict__ start,
+                                                    const int32_t *__restrict__ first, int n_tokens, int page_size, int max_pages,
+                                                    int num_pages) {
+    const int b = blockIdx.y, t = blockIdx.x * 128 + threadIdx.x;
+    if (t >= n_tokens) return;
+    const long long pos = (long long)start[b] + t, lp = pos / page_size;
+    if (pos < 0 || lp >= max_pages) return;
+    const int pg = table[(size_t)b * max_pages + lp];
+    if (pg < 0 || pg >= num_pages) { g_cache_error = ERR_PAGE; return; }
+    const size_t row = (size_t)pg * page_size + (size_t)(pos - lp * page_size);
+    weights[row] = 0.f;
+    positions[row] = first[b] + t;
+}
+
+// ---- evict, part 1: which rows stay ------------------------------------------------------------------------------------------
+// One cluster per sequence; CTA r holds the sort keys of its contiguous share of the rows in shared memory, read once.  The
+// keep-th largest key comes from three rounds of 11-, 11- and 10-bit histograms summed over the cluster; the ranks of equal
+// keys, evicted rows and moving rows from counts per warp (a warp owns a contiguous share of its CTA's rows).
+constexpr int SEL_THREADS = 1024, SEL_WARPS = SEL_THREADS / 32, BINS = 2048, MAX_CLUSTER = 16;
+constexpr int MAX_SEG = 49152;                   // rows per CTA: 192 KB of keys
+
+struct SelectProblem {
+    const float *weights;
+    const int32_t *positions;
+    Pages pg;
+    const int32_t *next;                         // [B] position of the next row to come
+    int32_t *kept;                               // [B, keep]: the row that row j held before, -1 past the end
+    int32_t *new_lens;                           // [B]
+    int32_t *movers;                             // [B, mover_cap] scratch: rows that move, in order
+    int keep, recent, seg, mover_cap;
+};
+
+__device__ __forceinline__ uint32_t sort_key(float w) {
+    if (isnan(w)) return 0u;                     // below everything
+    const uint32_t u = __float_as_uint(w + 0.f); // -0 counts as 0
+    return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+
+__device__ __forceinline__ void cluster_barrier(int cs) {
+    if (cs > 1) ptx::cluster_sync_all();
+    else __syncthreads();
+}
+
+struct SelShared {
+    uint32_t hist[BINS], total[BINS];
+    uint32_t warp_n[3][SEL_WARPS + 1];           // per warp: equal keys, evicted rows, moving rows; then their prefix sums
+    uint32_t cta_n[3];                           // of the whole CTA, read by the others
+    uint32_t base[3];                            // of the CTAs before this one
+    uint32_t scan[SEL_WARPS], prefix, remaining, digit;
+};
+
+// exclusive prefix sums over the CTA's warps and over the CTAs of the cluster of count `c` (already in sh.warp_n[c])
+__device__ __forceinline__ void ranks(SelShared &sh, int c, int rank, int cs) {
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        const uint32_t v = sh.warp_n[c][threadIdx.x];
+        uint32_t incl = v;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t u = __shfl_up_sync(0xffffffffu, incl, o);
+            if ((int)threadIdx.x >= o) incl += u;
+        }
+        sh.warp_n[c][threadIdx.x] = incl - v;
+        if (threadIdx.x == 31) sh.cta_n[c] = incl;
+    }
+    cluster_barrier(cs);
+    if (threadIdx.x == 0) {
+        uint32_t base = 0;
+        for (int r = 0; r < rank; ++r) base += ptx::ld_shared_cluster_u32(ptx::map_to_cta(ptx::smem_u32(&sh.cta_n[c]), r));
+        sh.base[c] = base;
+    }
+    __syncthreads();
+}
+
+__global__ void __launch_bounds__(SEL_THREADS, 1) select_kernel(const SelectProblem p, const int cs) {
+    extern __shared__ uint32_t s_key[];
+    __shared__ SelShared sh;
+    const int rank = cs > 1 ? (int)ptx::cluster_ctarank() : 0, b = blockIdx.x / cs;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int n = p.pg.length(b);
+    int32_t *kept = p.kept + (size_t)b * p.keep;
+    const int K = n < p.keep ? n : p.keep;
+    for (int j = rank * SEL_THREADS + tid; j < p.keep; j += cs * SEL_THREADS) kept[j] = j < K ? j : -1;
+    if (n <= p.keep) {                           // the whole cluster leaves: nothing goes
+        if (rank == 0 && tid == 0) p.new_lens[b] = n;
+        return;
+    }
+
+    const int lo = rank * p.seg < n ? rank * p.seg : n, hi = lo + p.seg < n ? lo + p.seg : n, rows = hi - lo;
+    const int newest = p.next[b] - p.recent;
+    for (int i = tid; i < rows; i += SEL_THREADS) {
+        const long long row = p.pg.row(b, lo + i);
+        uint32_t key = 0u;
+        if (row >= 0) key = p.positions[row] >= newest ? 0xffffffffu : sort_key(p.weights[row]);
+        s_key[i] = key;
+    }
+    if (tid == 0) { sh.prefix = 0u; sh.remaining = (uint32_t)K; }
+
+    // the K-th largest key, from the top digit down
+    for (int round = 0; round < 3; ++round) {
+        const int shift = round == 0 ? 21 : (round == 1 ? 10 : 0), bits = round == 2 ? 10 : 11, bins = 1 << bits;
+        for (int i = tid; i < BINS; i += SEL_THREADS) sh.hist[i] = 0u;
+        __syncthreads();
+        const uint32_t prefix = sh.prefix;
+        for (int i = tid; i < rows; i += SEL_THREADS) {
+            const uint32_t key = s_key[i];
+            if (round == 0 || (key >> (shift + bits)) == prefix) atomicAdd(&sh.hist[(key >> shift) & (bins - 1)], 1u);
+        }
+        cluster_barrier(cs);                     // every CTA's histogram stands
+        for (int i = tid; i < bins; i += SEL_THREADS) {
+            uint32_t v = 0;
+            if (cs == 1) v = sh.hist[i];
+            else for (int r = 0; r < cs; ++r) v += ptx::ld_shared_cluster_u32(ptx::map_to_cta(ptx::smem_u32(&sh.hist[i]), r));
+            sh.total[i] = v;
+        }
+        __syncthreads();
+        // thread i owns the two bins from the top; the digit is where the running count reaches what is still to be taken
+        const int hi_bin = bins - 1 - 2 * tid;
+        const uint32_t c0 = hi_bin >= 1 ? sh.total[hi_bin] : 0u, c1 = hi_bin >= 1 ? sh.total[hi_bin - 1] : 0u;
+        uint32_t incl = c0 + c1;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t u = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += u;
+        }
+        if (lane == 31) sh.scan[warp] = incl;
+        __syncthreads();
+        for (int w = 0; w < warp; ++w) incl += sh.scan[w];
+        const uint32_t before = incl - c0 - c1, want = sh.remaining;
+        __syncthreads();
+        if (before < want && want <= incl) {     // exactly one thread
+            const bool first = before + c0 >= want;
+            sh.prefix = (prefix << bits) | (uint32_t)(first ? hi_bin : hi_bin - 1);
+            sh.remaining = want - before - (first ? 0u : c0);
+        }
+        cluster_barrier(cs);                     // nobody clears a histogram that is still being read
+    }
+    const uint32_t T = sh.prefix, take = sh.remaining;       // of the keys equal to T the first `take` rows stay
+
+    // a warp owns rows [wlo, whi) of the CTA
+    const int per = ((rows + SEL_WARPS - 1) / SEL_WARPS + 31) & ~31;
+    const int wlo = warp * per < rows ? warp * per : rows, whi = wlo + per < rows ? wlo + per : rows;
+    uint32_t cnt = 0;
+    for (int i = wlo + lane; i < whi; i += 32) cnt += s_key[i] == T;
+    cnt = __reduce_add_sync(0xffffffffu, cnt);
+    if (lane == 0) sh.warp_n[0][warp] = cnt;
+    ranks(sh, 0, rank, cs);
+    const uint32_t eq0 = sh.base[0] + sh.warp_n[0][warp];
+    const uint32_t below = (1u << lane) - 1u;
+    for (int pass = 0; pass < 3; ++pass) {       // 0: count, 1: movers write their rows, 2: evicted rows take them
+        uint32_t eq = eq0;
+        uint32_t holes = 0, moves = 0;
+        if (pass > 0) { holes = sh.base[1] + sh.warp_n[1][warp]; moves = sh.base[2] + sh.warp_n[2][warp]; }
+        for (int i0 = wlo; i0 < whi; i0 += 32) {
+            const int i = i0 + lane, t = lo + i;
+            const bool live = i < whi;
+            const uint32_t key = live ? s_key[i] : 0u;
+            const uint32_t eqs = __ballot_sync(0xffffffffu, live && key == T);
+            const bool stays = live && (key > T || (key == T && eq + __popc(eqs & below) < take));
+            const uint32_t hole = __ballot_sync(0xffffffffu, live && t < K && !stays);
+            const uint32_t move = __ballot_sync(0xffffffffu, live && t >= K && stays);
+            if (pass == 1 && ((move >> lane) & 1u)) p.movers[(size_t)b * p.mover_cap + moves + __popc(move & below)] = t;
+            if (pass == 2 && ((hole >> lane) & 1u)) kept[t] = __ldcg(p.movers + (size_t)b * p.mover_cap + holes + __popc(hole & below));
+            eq += __popc(eqs);
+            holes += __popc(hole);
+            moves += __popc(move);
+        }
+        if (pass == 0) {
+            if (lane == 0) { sh.warp_n[1][warp] = holes; sh.warp_n[2][warp] = moves; }
+            ranks(sh, 1, rank, cs);
+            ranks(sh, 2, rank, cs);
+        } else if (pass == 1) {
+            __threadfence();
+            cluster_barrier(cs);                 // the list of movers stands; also: nobody leaves while its counts are read
+        }
+    }
+    if (rank == 0 && tid == 0) p.new_lens[b] = K;            // last: it may be the array the lengths were read from
+}
+
+// ---- evict, part 2: the copies -----------------------------------------------------------------------------------------------
+// A warp takes 32 places j at a time, reads what goes there (kept) and copies the rows that change place, two at a time.
+template <typename V>
+__global__ void __launch_bounds__(256) move_kernel(uint8_t *__restrict__ pool, float *__restrict__ weights,
+                                                   int32_t *__restrict__ positions, const int32_t *__restrict__ kept, const Pages pg,
+                                                   int B, int keep, int row_bytes) {
+    const int lane = threadIdx.x & 31;
+    const int groups = (keep + 31) / 32;
+    const long long warps = (long long)gridDim.x * 8;
+    const int vecs = row_bytes / (int)sizeof(V);
+    for (long long g = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); g < (long long)B * groups; g += warps) {
+        const int b = (int)(g / groups), j = (int)(g - (long long)b * groups) * 32 + lane;
+        const int src = j < keep ? kept[(size_t)b * keep + j] : -1;
+        long long from = -1, to = -1;
+        if (src >= 0 && src != j) {
+            from = pg.row(b, src);
+            to = pg.row(b, j);
+        }
+        const bool moves = from >= 0 && to >= 0;
+        if (moves) {
+            weights[to] = weights[from];
+            positions[to] = positions[from];
+        }
+        uint32_t todo = __ballot_sync(0xffffffffu, moves);
+        while (todo) {
+            const int a = __ffs(todo) - 1;
+            todo &= todo - 1;
+            const int c = todo ? __ffs(todo) - 1 : a;
+            todo &= todo ? todo - 1 : 0u;
+            const V *f0 = reinterpret_cast<const V *>(pool + __shfl_sync(0xffffffffu, from, a) * row_bytes);
+            const V *f1 = reinterpret_cast<const V *>(pool + __shfl_sync(0xffffffffu, from, c) * row_bytes);
+            V *d0 = reinterpret_cast<V *>(pool + __shfl_sync(0xffffffffu, to, a) * row_bytes);
+            V *d1 = reinterpret_cast<V *>(pool + __shfl_sync(0xffffffffu, to, c) * row_bytes);
+            for (int v = lane; v < vecs; v += 32) {
+                const V x = f0[v], y = f1[v];
+                d0[v] = x;
+                if (c != a) d1[v] = y;
+            }
+        }
+    }
+}
+
+}  // namespace cw
+
+int cache_error_flag(int reset) {
+    int v = 0;
+    if (cudaMemcpyFromSymbol(&v, cw::g_cache_error, sizeof(int)) != cudaSuccess) return -1;
+    if (reset && v != 0) {
+        const int zero = 0;
+        if (cudaMemcpyToSymbol(cw::g_cache_error, &zero, sizeof(int)) != cudaSuccess) return -1;
+    }
+    return v;
+}
+
+}  // namespace fdmla
+
+using namespace fdmla;
+
+static bool pages_ok(int B, int page_size, int max_pages, int num_pages) {
+    return B <= 65535 && (long long)page_size * max_pages <= 2147483647LL && (long long)page_size * num_pages <= 2147483647LL;
+}
+
+extern "C" size_t fdmla_cache_accumulate_workspace_bytes(int B, int H, int Sq, int d_qk, int page_size, int max_pages, int dtype) {
+    (void)B; (void)H; (void)Sq; (void)d_qk; (void)page_size; (void)max_pages; (void)dtype;
+    return 0;
+}
+
+extern "C" int fdmla_cache_accumulate(const void *Q, const void *kv_pool, const int32_t *page_table, const int32_t *seqlens,
+                                      const float *m, const float *l, float *weights, void *workspace, size_t workspace_bytes,
+                                      int B, int H, int Sq, int d_qk, int page_size, int max_pages, int num_pages, float scale,
+                                      int causal, int dtype, void *stream) {
+    if (B < 0 || H < 0 || Sq < 0 || d_qk <= 0 || page_size <= 0 || max_pages < 0 || num_pages < 0) return FDMLA_ERR_INVALID;
+    if (dtype != FDMLA_F32 && dtype != FDMLA_BF16) return FDMLA_ERR_INVALID;
+    if (B == 0 || H == 0 || Sq == 0 || max_pages == 0) return FDMLA_OK;
+    if (!Q || !kv_pool || !page_table || !seqlens || !m || !l || !weights) return FDMLA_ERR_INVALID;
+    if (!pages_ok(B, page_size, max_pages, num_pages) || (long long)H * Sq > 2147483647LL) return FDMLA_ERR_UNSUPPORTED;
+    if (workspace_bytes < fdmla_cache_accumulate_workspace_bytes(B, H, Sq, d_qk, page_size, max_pages, dtype)) return FDMLA_ERR_WORKSPACE;
+    (void)workspace;
+    cw::AccProblem p{};
+    p.Q = Q; p.pool = kv_pool; p.m = m; p.l = l; p.weights = weights;
+    p.pg = cw::Pages{page_table, seqlens, page_size, max_pages, num_pages};
+    p.B = B; p.R = H * Sq; p.Sq = Sq; p.d = d_qk; p.causal = causal ? 1 : 0;
+    p.scale_log2 = scale * 1.4426950408889634f;
+    cudaStream_t s = (cudaStream_t)stream;
+    if (fdmla_get_backend() == FDMLA_BACKEND_TENSOR) return FDMLA_ERR_UNSUPPORTED;
+    note_kernel("portable");
+    const long long smem = 32LL * (d_qk + 1) * 4;
+    if (smem > kMaxSmemPerBlock) return FDMLA_ERR_UNSUPPORTED;
+    const dim3 grid((unsigned)(((long long)max_pages * page_size + 31) / 32), B);
+    const void *fn = dtype == FDMLA_F32 ? (const void *)cw::accumulate_simt_kernel<float> : (const void *)cw::accumulate_simt_kernel<__nv_bfloat16>;
+    if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmemPerBlock) != cudaSuccess) { cudaGetLastError(); return FDMLA_ERR_CUDA; }
+    if (dtype == FDMLA_F32) cw::accumulate_simt_kernel<float><<<grid, cw::ACC_WARPS * 32, (size_t)smem, s>>>(p);
+    else cw::accumulate_simt_kernel<__nv_bfloat16><<<grid, cw::ACC_WARPS * 32, (size_t)smem, s>>>(p);
+    return check_launch();
+}
+
+extern "C" int fdmla_cache_stamp(float *weights, int32_t *positions, const int32_t *page_table, const int32_t *start_pos,
+                                 const int32_t *first_position, int B, int n_tokens, int page_size, int max_pages, int num_pages,
+                                 void *stream) {
+    if (B < 0 || n_tokens < 0 || page_size <= 0 || max_pages < 0 || num_pages < 0) return FDMLA_ERR_INVALID;
+    if (B == 0 || n_tokens == 0) return FDMLA_OK;
+    if (!weights || !positions || !page_table || !start_pos || !first_position) return FDMLA_ERR_INVALID;
+    if (!pages_ok(B, page_size, max_pages, num_pages)) return FDMLA_ERR_UNSUPPORTED;
+    cw::stamp_kernel<<<dim3((n_tokens + 127) / 128, B), 128, 0, (cudaStream_t)stream>>>(weights, positions, page_table, start_pos,
+                                                                                       first_position, n_tokens, page_size, max_pages, num_pages);
+    return check_launch();
+}
+
+extern "C" size_t fdmla_cache_evict_workspace_bytes(int B, int keep, int page_size, int max_pages) {
+    if (B <= 0 || keep <= 0 || page_size <= 0 || max_pages <= 0) return 0;
+    const long long cap = (long long)page_size * max_pages, movers = keep < cap ? keep : cap;
+    return (size_t)B * movers * sizeof(int32_t);
+}
+
+extern "C" int fdmla_cache_evict(void *kv_pool, float *weights, int32_t *positions, const int32_t *page_table,
+                                 const int32_t *seqlens, const int32_t *next_position, int32_t *kept, int32_t *new_seqlens,
+                                 void *workspace, size_t workspace_bytes, int B, int keep, int recent, int d_qk, int page_size,
+                                 int max_pages, int num_pages, int dtype, void *stream) {
+    if (B < 0 || keep <= 0 || recent < 0 || recent > keep || d_qk <= 0 || page_size <= 0 || max_pages < 0 || num_pages < 0) return FDMLA_ERR_INVALID;
+    if (dtype != FDMLA_F32 && dtype != FDMLA_BF16) return FDMLA_ERR_INVALID;
+    if (B == 0) return FDMLA_OK;
+    if (!kv_pool || !weights || !positions || !page_table || !seqlens || !next_position || !kept || !new_seqlens) return FDMLA_ERR_INVALID;
+    if (!pages_ok(B, page_size, max_pages, num_pages)) return FDMLA_ERR_UNSUPPORTED;
+    if (max_pages > 0 && (!workspace || workspace_bytes < fdmla_cache_evict_workspace_bytes(B, keep, page_size, max_pages))) return FDMLA_ERR_WORKSPACE;
+    cudaStream_t s = (cudaStream_t)stream;
+    const int cap = page_size * max_pages;
+    // CTAs per sequence: enough for every SM as long as a CTA keeps a few thousand rows, and room for the keys of the longest
+    int cs = 1;
+    while (cs < cw::MAX_CLUSTER && ((cap + cs - 1) / cs > cw::MAX_SEG - 32 || ((long long)B * cs * 2 <= kNumSMs && cap / cs > 4096))) cs *= 2;
+    const int seg = (((cap + cs - 1) / cs) + 31) & ~31;
+    if (seg > cw::MAX_SEG) return FDMLA_ERR_UNSUPPORTED;
+    cw::SelectProblem p{};
+    p.weights = weights; p.positions = positions;
+    p.pg = cw::Pages{page_table, seqlens, page_size, max_pages, num_pages};
+    p.next = next_position; p.kept = kept; p.new_lens = new_seqlens; p.movers = static_cast<int32_t *>(workspace);
+    p.keep = keep; p.recent = recent; p.seg = seg; p.mover_cap = keep < cap ? keep : cap;
+    const size_t smem = (size_t)seg * 4;
+    if (cudaFuncSetAttribute(cw::select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, cw::MAX_SEG * 4) != cudaSuccess ||
+        (cs > 8 && cudaFuncSetAttribute(cw::select_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)) {
+        cudaGetLastError();
+        return FDMLA_ERR_CUDA;
+    }
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)B * cs);
+    cfg.blockDim = dim3(cw::SEL_THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = cs; at.val.clusterDim.y = 1; at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    if (cudaLaunchKernelEx(&cfg, cw::select_kernel, p, cs) != cudaSuccess) { cudaGetLastError(); return FDMLA_ERR_CUDA; }
+    if (cap <= keep) return check_launch();                   // no sequence can be over its bound
+    const int row_bytes = d_qk * (dtype == FDMLA_F32 ? 4 : 2);
+    const long long warps = (long long)B * ((keep + 31) / 32);
+    const unsigned blocks = (unsigned)(warps > 8LL * 8 * kNumSMs ? 8 * kNumSMs : (warps + 7) / 8);
+    uint8_t *pool = static_cast<uint8_t *>(kv_pool);
+    if (row_bytes % 16 == 0 && (reinterpret_cast<uintptr_t>(kv_pool) & 15) == 0)
+        cw::move_kernel<uint4><<<blocks, 256, 0, s>>>(pool, weights, positions, kept, p.pg, B, keep, row_bytes);
+    else if (row_bytes % 4 == 0)
+        cw::move_kernel<uint32_t><<<blocks, 256, 0, s>>>(pool, weights, positions, kept, p.pg, B, keep, row_bytes);
+    else
+        cw::move_kernel<uint16_t><<<blocks, 256, 0, s>>>(pool, weights, positions, kept, p.pg, B, keep, row_bytes);
+    return check_launch();
+}

@@ -144,6 +144,7 @@ int launch_rope_rows(const void *x, long long ldx, void *y, long long ldy, const
                      int rows_per_pos, int d, float base, cudaStream_t stream);
 int gemm_error_flag(int reset);
 int exchange_error_flag(int reset);
+int cache_error_flag(int reset);          // bad page ids and lengths seen by the cache-weight kernels
 size_t exchange_bytes(int world, long long rows, int d_v);
 int launch_exchange_merge(const float *O_part, const float *m_part, const float *l_part, int num_parts, void *msg,
                           void *const *bufs, int world, int rank, long long rows, int d_v, void *O,
@@ -154,6 +155,8 @@ int launch_project_tensor(const void *X, const void *W, void *Y, long long rows,
                           int x_f32, cudaStream_t stream);
 int launch_wgrad_partial_tensor(const void *X, const float *G, float *part, long long rows, int d_in, int d_out, int n_part,
                                 cudaStream_t stream);
+// kernel family reported by fdmla_last_kernel for the calling thread ("tcgen05" or "portable")
+void note_kernel(const char *family);
 // false when the caller has forced the CUDA-core kernels (fdmla_set_backend)
 bool tensor_kernels_allowed();
 int wgrad_num_partials(long long rows);

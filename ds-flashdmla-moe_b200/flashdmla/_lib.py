@@ -54,6 +54,13 @@ SIGNATURES = {
     "fdmla_bwd_cache_latent": (_i, [_vp] * 9 + [_sz] + [_i] * 6 + [_f, _i, _i, _vp]),
     "fdmla_cache_append": (_i, [_vp] * 4 + [_i] * 7 + [_vp]),
     "fdmla_cache_gather": (_i, [_vp] * 4 + [_i] * 7 + [_vp]),
+    "fdmla_cache_stamp": (_i, [_vp] * 5 + [_i] * 5 + [_vp]),
+    "fdmla_cache_accumulate_workspace_bytes": (_sz, [_i] * 7),
+    "fdmla_cache_accumulate": (_i, [_vp] * 8 + [_sz] + [_i] * 7 + [_f, _i, _i, _vp]),
+    "fdmla_cache_evict_workspace_bytes": (_sz, [_i] * 4),
+    "fdmla_cache_evict": (_i, [_vp] * 9 + [_sz] + [_i] * 8 + [_vp]),
+    "fdmla_moe_few_workspace_bytes": (_sz, [_i] * 7),
+    "fdmla_moe_few": (_i, [_vp] * 10 + [_sz] + [_i] * 6 + [_vp]),
     "fdmla_moe_route_topk": (_i, [_vp] * 3 + [_i] * 3 + [_vp]),
     "fdmla_moe_pack_workspace_bytes": (_sz, [_i] * 3),
     "fdmla_moe_pack": (_i, [_vp] * 5 + [_sz] + [_i] * 5 + [_vp]),

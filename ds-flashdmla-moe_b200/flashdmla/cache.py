@@ -12,6 +12,14 @@ host-side page allocator:
     O, m, l = cache.decode(Q, [slot], d_v=512, scale=...)
     cache.free_sequence(slot)
 
+With track_weights=True the cache can be bounded: beside every row it keeps the attention weight the row has received
+(added by `decode`) and the position of its token, and
+
+    cache.evict(slots, keep=4096, recent=128)   # at most 4096 rows each: the newest 128 and the heaviest others
+
+gives the pages behind row `keep` back.  Rows are then no longer in the order of their tokens (the attention does not
+depend on it); `position(slot)` is the position of the next token, `length(slot)` the number of rows held.
+
 Page bookkeeping (free list, lengths, the host copy of the page table) is plain Python and
 runs without a GPU (`device="cpu"`: the pool then only exists as metadata and `append`
 needs `rows=None`); the row copies and the attention run through the CUDA library.
@@ -28,7 +36,7 @@ from ._lib import FlashDMLAError
 
 class PagedLatentCache:
     def __init__(self, num_pages: int, page_size: int, d_qk: int, max_seqs: int, max_pages_per_seq: int,
-                 dtype: torch.dtype = torch.bfloat16, device="cuda"):
+                 dtype: torch.dtype = torch.bfloat16, device="cuda", track_weights: bool = False):
         if num_pages <= 0 or page_size <= 0 or d_qk <= 0 or max_seqs <= 0 or max_pages_per_seq <= 0:
             raise FlashDMLAError("cache dimensions must be positive")
         self.num_pages, self.page_size, self.d_qk = int(num_pages), int(page_size), int(d_qk)
@@ -36,9 +44,15 @@ class PagedLatentCache:
         self.device = torch.device(device)
         self.on_gpu = self.device.type == "cuda"
         self.pool = (torch.zeros(num_pages, page_size, d_qk, dtype=dtype, device=self.device) if self.on_gpu else None)
+        self.track_weights = bool(track_weights)
+        self.weights = self.positions = None
+        if self.on_gpu and self.track_weights:
+            self.weights = torch.zeros(num_pages, page_size, dtype=torch.float32, device=self.device)
+            self.positions = torch.full((num_pages, page_size), -1, dtype=torch.int32, device=self.device)
         # host truth, device mirror (the kernels read the mirror)
         self.h_table = torch.zeros(max_seqs, max_pages_per_seq, dtype=torch.int32)
         self.h_len = torch.zeros(max_seqs, dtype=torch.int32)
+        self.h_next = torch.zeros(max_seqs, dtype=torch.int32)                 # position of the next token
         self.d_table = self.h_table.to(self.device) if self.on_gpu else None
         self.d_len = self.h_len.to(self.device) if self.on_gpu else None
         self._free_pages: List[int] = list(range(num_pages - 1, -1, -1))      # pop() hands out page 0 first
@@ -55,6 +69,11 @@ class PagedLatentCache:
         self._check_slot(slot)
         return int(self.h_len[slot])
 
+    def position(self, slot: int) -> int:
+        """Position of the next token of the sequence: the tokens appended so far, evicted ones included."""
+        self._check_slot(slot)
+        return int(self.h_next[slot])
+
     def pages_of(self, slot: int) -> List[int]:
         self._check_slot(slot)
         return list(self._pages_of[slot])
@@ -65,6 +84,7 @@ class PagedLatentCache:
         slot = self._free_slots.pop()
         self._live[slot] = True
         self.h_len[slot] = 0
+        self.h_next[slot] = 0
         return slot
 
     def free_sequence(self, slot: int) -> None:
@@ -72,6 +92,7 @@ class PagedLatentCache:
         self._free_pages.extend(reversed(self._pages_of[slot]))
         self._pages_of[slot] = []
         self.h_len[slot] = 0
+        self.h_next[slot] = 0
         self.h_table[slot].zero_()
         self._live[slot] = False
         self._free_slots.append(slot)
@@ -103,6 +124,7 @@ class PagedLatentCache:
                 self._pages_of[s].append(pg)
             start[i] = self.h_len[s]
             self.h_len[s] += n_tokens
+            self.h_next[s] += n_tokens
         self._sync_rows(slots)
         return start
 
@@ -116,9 +138,13 @@ class PagedLatentCache:
             raise FlashDMLAError("rows must be [len(slots), n_tokens, d_qk]")
         if not self.on_gpu:
             raise FlashDMLAError("append needs a CUDA cache (there is no CPU fallback)")
+        first = torch.tensor([self.position(s) for s in slots], dtype=torch.int32)
         start = self.reserve(slots, rows.shape[1])
         idx = torch.tensor(list(slots), dtype=torch.long, device=self.device)
-        ops.cache_append(rows, self.pool, self.d_table.index_select(0, idx), start.to(self.device))
+        table, d_start = self.d_table.index_select(0, idx), start.to(self.device)
+        ops.cache_append(rows, self.pool, table, d_start)
+        if self.track_weights:
+            ops.cache_stamp(self.weights, self.positions, table, d_start, first.to(self.device), rows.shape[1])
         return start
 
     def tables(self, slots: Sequence[int]):
@@ -128,17 +154,65 @@ class PagedLatentCache:
         idx = torch.tensor(list(slots), dtype=torch.long, device=self.device)
         return self.d_table.index_select(0, idx), self.d_len.index_select(0, idx)
 
-    def decode(self, Q: torch.Tensor, slots: Sequence[int], d_v: int, scale: Optional[float] = None, **kw):
-        """One decode step of the listed sequences: Q [len(slots), H, d_qk] -> (O, m, l)."""
+    def decode(self, Q: torch.Tensor, slots: Sequence[int], d_v: int, scale: Optional[float] = None,
+               accumulate: Optional[bool] = None, **kw):
+        """One decode step of the listed sequences: Q [len(slots), H, d_qk] -> (O, m, l).  A cache that tracks weights also
+        adds the attention weight every row received in this step, unless accumulate=False."""
+        if accumulate is None:
+            accumulate = self.track_weights
+        if accumulate and not self.track_weights:
+            raise FlashDMLAError("this cache does not track weights (track_weights=True)")
+        if accumulate and (kw.get("partial_only") or kw.get("kv_begin", 0) > 0 or kw.get("kv_end", -1) >= 0):
+            raise FlashDMLAError("weights are accumulated over whole sequences: pass accumulate=False with a key window or partial_only")
+        if accumulate and len(set(slots)) != len(slots):
+            raise FlashDMLAError("a sequence may appear only once per step")
         table, lens = self.tables(slots)
         longest = max((int(self.h_len[s]) for s in slots), default=0)
-        return ops.flash_dmla_paged_decode(Q, self.pool, table, lens, d_v, scale, max_seqlen=max(longest, 1), **kw)
+        out = ops.flash_dmla_paged_decode(Q, self.pool, table, lens, d_v, scale, max_seqlen=max(longest, 1), **kw)
+        if accumulate:
+            ops.accumulate_weights(Q, self.pool, table, lens, out[1], out[2], self.weights, scale)
+        return out
+
+    def evict(self, slots: Sequence[int], keep: int, recent: int = 0) -> torch.Tensor:
+        """Cut every listed sequence with more than `keep` rows to `keep`: the rows of the newest `recent` positions stay,
+        then those of the largest accumulated weight (`ops.cache_evict`).  Pages behind row `keep` become free.  Returns
+        kept [len(slots), keep] int32 on the device: the row that row j held before, -1 past the end."""
+        if not self.on_gpu or not self.track_weights:
+            raise FlashDMLAError("evict needs a CUDA cache with track_weights=True")
+        if len(set(slots)) != len(slots):
+            raise FlashDMLAError("a sequence may appear only once per eviction")
+        table, lens = self.tables(slots)
+        nxt = torch.tensor([self.position(s) for s in slots], dtype=torch.int32).to(self.device)
+        kept, _ = ops.cache_evict(self.pool, self.weights, self.positions, table, lens, nxt, keep, recent)
+        self._shrink(slots, int(keep))
+        return kept
+
+    def row_state(self, slot: int):
+        """(weights, positions) of a sequence's rows, in the order of the rows."""
+        self._check_slot(slot)
+        if not self.on_gpu or not self.track_weights:
+            raise FlashDMLAError("row_state needs a CUDA cache with track_weights=True")
+        n = int(self.h_len[slot])
+        pages = torch.tensor(self._pages_of[slot], dtype=torch.long, device=self.device)
+        return self.weights[pages].flatten()[:n], self.positions[pages].flatten()[:n]
 
     def gather(self, slots: Sequence[int], n_tokens: int) -> torch.Tensor:
         table, lens = self.tables(slots)
         return ops.cache_gather(self.pool, table, lens, n_tokens)
 
     # ------------------------------------------------------------------ helpers
+    def _shrink(self, slots: Sequence[int], keep: int) -> None:
+        """Lengths at most `keep`, pages no longer needed back to the free list."""
+        for s in slots:
+            self._check_slot(s)
+            self.h_len[s] = min(int(self.h_len[s]), keep)
+            need = (int(self.h_len[s]) + self.page_size - 1) // self.page_size
+            spare = self._pages_of[s][need:]
+            self._free_pages.extend(reversed(spare))
+            self._pages_of[s] = self._pages_of[s][:need]
+            self.h_table[s, need:] = 0
+        self._sync_rows(slots)
+
     def _check_slot(self, slot: int) -> None:
         if not (0 <= slot < self.max_seqs) or not self._live[slot]:
             raise FlashDMLAError(f"sequence slot {slot} is not live")

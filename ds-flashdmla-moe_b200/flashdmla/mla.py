@@ -80,7 +80,7 @@ class AbsorbedMLA:
 
     def decode(self, cache: PagedLatentCache, slots: Sequence[int], h: torch.Tensor) -> torch.Tensor:
         """Append the new token of every listed sequence and attend: h [n, d_model] -> [n, d_model]."""
-        pos = torch.tensor([cache.length(s) for s in slots], device=h.device)
+        pos = torch.tensor([cache.position(s) for s in slots], device=h.device)
         cache.append(slots, self.cache_rows(h[:, None, :], pos[:, None]))
         o_lat, _, _ = cache.decode(self.absorbed_query(h, pos), slots, self.d_lat, self.scale)
         from . import gemm

@@ -7,7 +7,8 @@ the reference describes at README.md:17-20, and its single-node expert paralleli
     yp              = expert MLP on xp[offs[e]:offs[e+1]]    # plain GEMMs (torch.matmul = vendor library)
     out             = combine(yp, pos, w, shared)            # renormalised weights, shared expert added
 
-`MoEFFN.forward` runs that on one GPU.  `MoEFFN.forward_ep` shards the experts over the ranks of a
+`MoEFFN.forward` runs that on one GPU, `MoEFFN.forward_few` (`moe_few`) the same layer for the few tokens of a
+decode step in two launches, without a capacity.  `MoEFFN.forward_ep` shards the experts over the ranks of a
 process group (one process per GPU): packed rows are ordered by expert, so the rows for rank r's
 experts are one contiguous range; counts and rows are exchanged with `all_to_all_single`, every
 rank runs its own experts, and the results travel back the same way.  Forward only.
@@ -99,6 +100,50 @@ def combine(y: torch.Tensor, pos: torch.Tensor, w: torch.Tensor, shared: Optiona
     return out
 
 
+MAX_FEW_TOKENS = 128
+
+
+def moe_few(x: torch.Tensor, Wg: torch.Tensor, W1: torch.Tensor, W3: torch.Tensor, W2: torch.Tensor, k: int,
+            shared: Optional[Sequence[torch.Tensor]] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The whole layer for the few tokens of a decode step (at most MAX_FEW_TOKENS): x [T,d], Wg [d,E] fp32, W1, W3 [E,d,f],
+    W2 [E,f,d], shared = (S1 [d,f], S3 [d,f], S2 [f,d]) or None -> [T,d] in x's dtype.
+
+    The k experts with the largest logit win (ties: the lower expert), their outputs are weighted with the softmax over the
+    winners' logits; there is no capacity and nothing is dropped.  Every chosen expert's weights are read once.  Weights have
+    to be finite.  out: a contiguous tensor to write into."""
+    _need_cuda(x, Wg, W1, W3, W2, *(shared or ()))
+    if x.dim() != 2 or Wg.dim() != 2 or W1.dim() != 3 or W2.dim() != 3:
+        raise FlashDMLAError("expected x [T,d], Wg [d,E], W1, W3 [E,d,f], W2 [E,f,d]")
+    (T, d), (E, _, f) = x.shape, W1.shape
+    if tuple(Wg.shape) != (d, E) or tuple(W1.shape) != (E, d, f) or W3.shape != W1.shape or tuple(W2.shape) != (E, f, d):
+        raise FlashDMLAError("shape mismatch between x, Wg, W1, W3 and W2")
+    if Wg.dtype != torch.float32:
+        raise FlashDMLAError("the gate weights must be float32")
+    if any(t.dtype != x.dtype for t in (W1, W3, W2, *(shared or ()))):
+        raise FlashDMLAError("x and the expert weights must share one dtype")
+    if shared is not None and [tuple(t.shape) for t in shared] != [(d, f), (d, f), (f, d)]:
+        raise FlashDMLAError("the shared expert must be (S1 [d,f], S3 [d,f], S2 [f,d])")
+    if T > MAX_FEW_TOKENS:
+        raise FlashDMLAError(f"moe_few takes at most {MAX_FEW_TOKENS} tokens, got {T}")
+    k = int(k)
+    if not 1 <= k <= min(E, 32):
+        raise FlashDMLAError("k must be between 1 and min(E, 32)")
+    x, Wg, W1, W3, W2 = (t.contiguous() for t in (x, Wg, W1, W3, W2))
+    S1, S3, S2 = (t.contiguous() for t in shared) if shared is not None else (None, None, None)
+    if out is None:
+        out = torch.empty(T, d, dtype=x.dtype, device=x.device)
+    elif tuple(out.shape) != (T, d) or out.dtype != x.dtype or out.device != x.device or not out.is_contiguous():
+        raise FlashDMLAError("out must be a contiguous [T,d] tensor of x's dtype on its GPU")
+    code = _dtype_code(x)
+    with torch.cuda.device(x.device):
+        L = _lib.lib()
+        nbytes = L.fdmla_moe_few_workspace_bytes(T, d, f, E, k, int(shared is not None), code)
+        ws = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=x.device)
+        check(L.fdmla_moe_few(_ptr(x), _ptr(Wg), _ptr(W1), _ptr(W3), _ptr(W2), _ptr(S1), _ptr(S3), _ptr(S2), _ptr(out),
+                              _ptr(ws), ws.numel(), T, d, f, E, k, code, _stream(x)), "fdmla_moe_few")
+    return out
+
+
 def swiglu_mlp(x, W1, W3, W2):
     """(silu(x W1) * (x W3)) W2 with library GEMMs."""
     return (torch.nn.functional.silu(x @ W1) * (x @ W3)) @ W2
@@ -160,6 +205,11 @@ class MoEFFN:
         yp = gemm.expert_mlp_grouped(xp, offsets, self.W1, self.W3, self.W2)
         sh = swiglu_mlp(x, *self.shared) if self.shared is not None else None
         return combine(yp, pos, w, sh)
+
+    def forward_few(self, x: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """x [T,d] -> [T,d] for the few tokens of a decode step (at most MAX_FEW_TOKENS), all experts on this GPU: one call of
+        `moe_few`.  Unlike `forward` it has no capacity, so no token loses an expert."""
+        return moe_few(x, self.Wg, self.W1, self.W3, self.W2, self.k, self.shared, out)
 
     def forward_batched(self, x: torch.Tensor, capacity: Optional[int] = None) -> torch.Tensor:
         """The same layer with padded packing: the packed rows are an [E, capacity, d] batch, the expert MLPs

@@ -426,3 +426,103 @@ def cache_gather(kv_pool, page_table, seqlens, n_tokens: int):
             int(n_tokens), d, page_size, page_table.shape[1], num_pages, _dtype_code(kv_pool),
             _stream(kv_pool)), "fdmla_cache_gather")
     return out
+
+
+# --------------------------------------------------------------------------- #
+# a cache that may not grow: attention weight per cached row, eviction
+# --------------------------------------------------------------------------- #
+def _check_tables(page_table, B, *per_seq) -> None:
+    if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != B:
+        raise FlashDMLAError("page_table must be [B, max_pages] int32")
+    for t in per_seq:
+        if t.dtype != torch.int32 or tuple(t.shape) != (B,):
+            raise FlashDMLAError("lengths and positions per sequence must be [B] int32")
+
+
+def _check_row_state(kv_pool, weights, positions=None) -> None:
+    if kv_pool.dim() != 3 or not kv_pool.is_contiguous():
+        raise FlashDMLAError("kv_pool must be a contiguous [num_pages, page_size, d_qk] tensor")
+    for t, dt, name in ((weights, torch.float32, "weights"), (positions, torch.int32, "positions")):
+        if t is None:
+            continue
+        if t.dtype != dt or tuple(t.shape) != tuple(kv_pool.shape[:2]) or not t.is_contiguous():
+            raise FlashDMLAError(f"{name} must be a contiguous [num_pages, page_size] {dt} tensor (it is written in place)")
+
+
+def cache_stamp(weights, positions, page_table, start_pos, first_position, n_tokens: int) -> None:
+    """Bookkeeping of new rows, the companion of `cache_append`: the n_tokens rows of sequence b from logical row
+    start_pos[b] on get weight 0 and positions first_position[b], first_position[b] + 1, ... (in place)."""
+    _need_cuda(weights, positions, page_table, start_pos, first_position)
+    _check_tables(page_table, page_table.shape[0], start_pos, first_position)
+    if weights.dtype != torch.float32 or positions.dtype != torch.int32 or weights.dim() != 2 or weights.shape != positions.shape \
+            or not weights.is_contiguous() or not positions.is_contiguous():
+        raise FlashDMLAError("weights (float32) and positions (int32) must be contiguous [num_pages, page_size] tensors")
+    num_pages, page_size = weights.shape
+    with torch.cuda.device(weights.device):
+        check(_lib.lib().fdmla_cache_stamp(_ptr(weights), _ptr(positions), _ptr(page_table.contiguous()),
+                                           _ptr(start_pos.contiguous()), _ptr(first_position.contiguous()), page_table.shape[0],
+                                           int(n_tokens), page_size, page_table.shape[1], num_pages, _stream(weights)),
+              "fdmla_cache_stamp")
+
+
+def accumulate_weights(Q, kv_pool, page_table, seqlens, m, l, weights, scale=None, causal=True):
+    """Add to every cached row the attention weight it receives from these queries, summed over heads and queries.
+
+    Q [B,H,d_qk] (a decode step) or [B,H,Sq,d_qk] (a prompt, or its last Sq queries); m, l of the attention of the same
+    queries over the same cache with the same scale, shaped like Q without its last dimension; weights
+    [num_pages,page_size] fp32, changed in place and returned.  causal: query i sees keys t <= i + seqlens[b] - Sq.
+    Queries that see nothing (l = 0) add nothing; the sequences of one call should not share pages."""
+    _need_cuda(Q, kv_pool, page_table, seqlens, m, l, weights)
+    _same_dtype(Q, kv_pool)
+    if Q.dim() not in (3, 4):
+        raise FlashDMLAError("Q must be [B,H,d_qk] or [B,H,Sq,d_qk]")
+    if m.dtype != torch.float32 or l.dtype != torch.float32 or m.shape != Q.shape[:-1] or l.shape != Q.shape[:-1]:
+        raise FlashDMLAError("m and l must be float32 with the shape of Q without its last dimension")
+    B, H = Q.shape[:2]
+    Sq, d_qk = (1 if Q.dim() == 3 else Q.shape[2]), Q.shape[-1]
+    _check_tables(page_table, B, seqlens)
+    _check_row_state(kv_pool, weights)
+    num_pages, page_size, d_pool = kv_pool.shape
+    if d_pool != d_qk:
+        raise FlashDMLAError("Q and kv_pool differ in their last dimension")
+    if scale is None:
+        scale = 1.0 / math.sqrt(d_qk)
+    Q, m, l, page_table, seqlens = (t.contiguous() for t in (Q, m, l, page_table, seqlens))
+    code, max_pages = _dtype_code(Q), page_table.shape[1]
+    with torch.cuda.device(Q.device):
+        L = _lib.lib()
+        nbytes = L.fdmla_cache_accumulate_workspace_bytes(B, H, Sq, d_qk, page_size, max_pages, code)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=Q.device) if nbytes else None
+        check(L.fdmla_cache_accumulate(_ptr(Q), _ptr(kv_pool), _ptr(page_table), _ptr(seqlens), _ptr(m), _ptr(l), _ptr(weights),
+                                       _ptr(ws), nbytes, B, H, Sq, d_qk, page_size, max_pages, num_pages, float(scale),
+                                       int(bool(causal)), code, _stream(Q)), "fdmla_cache_accumulate")
+    return weights
+
+
+def cache_evict(kv_pool, weights, positions, page_table, seqlens, next_position, keep: int, recent: int = 0):
+    """Cut every sequence with more than `keep` rows to `keep` (in place); returns kept [B,keep], new_seqlens [B] (int32).
+
+    Rows with position >= next_position[b] - recent stay, then the rows of the largest weight, ties: the lower row.
+    Survivors in front of row `keep` do not move, those behind it fill the evicted rows' places, both in ascending
+    order; weights and positions move with their rows.  kept[b,j] is the row that row j held before, -1 past the new
+    end.  Rows from `keep` on are left as they were.  The sequences of one call must not share pages."""
+    _need_cuda(kv_pool, weights, positions, page_table, seqlens, next_position)
+    _check_row_state(kv_pool, weights, positions)
+    B, keep, recent = page_table.shape[0], int(keep), int(recent)
+    _check_tables(page_table, B, seqlens, next_position)
+    if keep < 1 or not 0 <= recent <= keep:
+        raise FlashDMLAError("cache_evict needs keep >= 1 and 0 <= recent <= keep")
+    num_pages, page_size, d_qk = kv_pool.shape
+    max_pages, dev = page_table.shape[1], kv_pool.device
+    page_table, seqlens, next_position = page_table.contiguous(), seqlens.contiguous(), next_position.contiguous()
+    kept = torch.empty(B, keep, dtype=torch.int32, device=dev)
+    new_seqlens = torch.empty(B, dtype=torch.int32, device=dev)
+    with torch.cuda.device(dev):
+        L = _lib.lib()
+        nbytes = L.fdmla_cache_evict_workspace_bytes(B, keep, page_size, max_pages)
+        ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
+        check(L.fdmla_cache_evict(_ptr(kv_pool), _ptr(weights), _ptr(positions), _ptr(page_table), _ptr(seqlens),
+                                  _ptr(next_position), _ptr(kept), _ptr(new_seqlens), _ptr(ws), ws.numel(), B, keep, recent,
+                                  d_qk, page_size, max_pages, num_pages, _dtype_code(kv_pool), _stream(kv_pool)),
+              "fdmla_cache_evict")
+    return kept, new_seqlens

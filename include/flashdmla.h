@@ -402,6 +402,64 @@ int fdmla_cache_gather(const void *kv_pool, const int32_t *page_table,
                        int d_qk, int page_size, int max_pages, int num_pages,
                        int dtype, void *stream);
 
+/*
+ * A latent cache that may not grow.  Beside the pool stand, addressed through the same page table,
+ *   weights   [num_pages, page_size] fp32   attention weight every cached row has received so far
+ *   positions [num_pages, page_size] int32  position of the row's token in its sequence
+ * No counterpart in the reference (README.md:15 only names the cache).
+ *
+ * fdmla_cache_stamp: what fdmla_cache_append is to the rows - new tokens t of sequence b at logical row
+ * start_pos[b] + t get weight 0 and position first_position[b] + t.
+ */
+int fdmla_cache_stamp(float *weights, int32_t *positions,
+                      const int32_t *page_table, const int32_t *start_pos,
+                      const int32_t *first_position, int B, int n_tokens,
+                      int page_size, int max_pages, int num_pages, void *stream);
+
+/*
+ * weights[row of key t of sequence b] += sum over query rows (h, i) that see t of exp(scale q_hi . k_t - m_hi) / l_hi.
+ *   Q [B, H, Sq, d_qk] (Sq = 1: one decode step; Sq > 1: a prompt or its last Sq queries), m, l [B, H, Sq] fp32 as the
+ *   attention of the same step returned them for the same scale; query i sees keys t <= i + seqlens[b] - Sq when causal,
+ *   all seqlens[b] keys otherwise.  A query row with l <= 0 (nothing visible) gives nothing.
+ *   Sequences of one call should own their pages; if two share one, its weights receive both sums (in either order).
+ *   workspace: fdmla_cache_accumulate_workspace_bytes() bytes of device scratch, 256-byte aligned (may be 0 bytes: NULL).
+ *   bf16 with d_qk a multiple of 64 up to 576 and page_size a multiple of 64 runs on the tensor cores, everything else with
+ *   d_qk <= 1815 on CUDA cores.  Bad page ids and lengths are skipped / clamped and reported (code 4).
+ */
+size_t fdmla_cache_accumulate_workspace_bytes(int B, int H, int Sq, int d_qk,
+                                              int page_size, int max_pages,
+                                              int dtype);
+int fdmla_cache_accumulate(const void *Q, const void *kv_pool,
+                           const int32_t *page_table, const int32_t *seqlens,
+                           const float *m, const float *l, float *weights,
+                           void *workspace, size_t workspace_bytes, int B, int H,
+                           int Sq, int d_qk, int page_size, int max_pages,
+                           int num_pages, float scale, int causal, int dtype,
+                           void *stream);
+
+/*
+ * Eviction.  Every sequence with more than `keep` rows is cut to `keep`; shorter ones stay as they are.
+ *   Which rows stay: first those with position >= next_position[b] - recent, then by descending weight; ties: the lower
+ *   row.  A NaN weight counts as less than every number.
+ *   Where they are afterwards: survivors in front of row `keep` do not move; the survivors behind it, in ascending order,
+ *   take the places of the evicted rows in front of it, in ascending order - in the pool, in weights and in positions.
+ *   Rows from `keep` on keep their contents.
+ *   kept [B, keep] int32 (out): the row that row j held before the call, -1 for j past the new end.
+ *   new_seqlens [B] int32 (out): min(seqlens[b], keep); may be the array seqlens itself.
+ *   0 <= recent <= keep, keep >= 1.  The sequences of one call must not share pages.  page_size * max_pages at most
+ *   785 000 rows (FDMLA_ERR_UNSUPPORTED beyond).  A row on a bad page counts as the lightest and is not copied (code 4).
+ *   workspace: fdmla_cache_evict_workspace_bytes() bytes of device scratch.
+ */
+size_t fdmla_cache_evict_workspace_bytes(int B, int keep, int page_size,
+                                         int max_pages);
+int fdmla_cache_evict(void *kv_pool, float *weights, int32_t *positions,
+                      const int32_t *page_table, const int32_t *seqlens,
+                      const int32_t *next_position, int32_t *kept,
+                      int32_t *new_seqlens, void *workspace,
+                      size_t workspace_bytes, int B, int keep, int recent,
+                      int d_qk, int page_size, int max_pages, int num_pages,
+                      int dtype, void *stream);
+
 /* --------------------------------------------------------------------------
  * MoE FFN plumbing (the "unfused reference path" of README.md:17-20: Top-K gate
  * -> per-expert packing (bucket + exclusive scan) -> expert MLP -> combine and
@@ -465,6 +523,26 @@ int fdmla_moe_scatter(const void *x, const int32_t *pos, void *packed, int T,
 int fdmla_moe_combine(const void *y, const int32_t *pos, const float *w,
                       const void *shared, void *out, int T, int k, int d,
                       int dtype, void *stream);
+
+/*
+ * The whole MoE FFN layer for the few tokens of a decode step, T <= 128: gate, top-k, the chosen experts' SwiGLU MLPs, the
+ * shared expert and the weighted sum.
+ *   z = x Wg; the k experts with the largest z win (ties: lower expert); w = softmax over the k winners' z
+ *   out[t] = sum_j w[t, j] (silu(x[t] W1[e_j]) * (x[t] W3[e_j])) W2[e_j]  + (silu(x[t] S1) * (x[t] S3)) S2
+ *   x [T, d], Wg [d, E] fp32, W1, W3 [E, d, f], W2 [E, f, d], shared expert S1, S3 [d, f], S2 [f, d] (all three NULL: none),
+ *   out [T, d]; x, W*, S*, out in `dtype`.  There is no capacity: nothing is dropped.
+ *   The logits are summed in 64 bits.  bf16 with d and f multiples of 64 runs on the tensor cores: the intermediate
+ *   activation, gate weight included, is rounded to bf16 once, sums are fp32, out is rounded once.  An expert that any token
+ *   of the call chooses multiplies all of the call's tokens with zeros for the others: weights must be finite there.
+ *   Everything else runs on CUDA cores with an fp32 intermediate.
+ *   k <= min(E, 32), E <= 2048; workspace: fdmla_moe_few_workspace_bytes() bytes of device scratch, 256-byte aligned.
+ */
+size_t fdmla_moe_few_workspace_bytes(int T, int d, int f, int E, int k,
+                                     int shared, int dtype);
+int fdmla_moe_few(const void *x, const float *Wg, const void *W1, const void *W3,
+                  const void *W2, const void *S1, const void *S3, const void *S2,
+                  void *out, void *workspace, size_t workspace_bytes, int T,
+                  int d, int f, int E, int k, int dtype, void *stream);
 
 #ifdef __cplusplus
 }
