@@ -142,8 +142,8 @@ int fdmla_set_single_cta(int on) { tensor_prefer_single_cta(on != 0); return FDM
 const char *fdmla_last_kernel(void) { return t_last_kernel; }
 int fdmla_device_error_flag(int reset) {
     const int fwd = tensor_error_flag(reset), bwd = bwd_tensor_error_flag(reset), gemm = gemm_error_flag(reset),
-              xch = exchange_error_flag(reset), cache = cache_error_flag(reset);
-    return fwd ? fwd : (bwd ? bwd : (gemm ? gemm : (xch ? xch : cache)));
+              xch = exchange_error_flag(reset), few = few_error_flag(reset), cache = cache_error_flag(reset);
+    return fwd ? fwd : (bwd ? bwd : (gemm ? gemm : (xch ? xch : (few ? few : cache))));
 }
 
 size_t fdmla_exchange_bytes(int world, long long rows, int d_v) { return exchange_bytes(world, rows, d_v); }

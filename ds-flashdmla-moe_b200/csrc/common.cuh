@@ -144,6 +144,7 @@ int launch_rope_rows(const void *x, long long ldx, void *y, long long ldy, const
                      int rows_per_pos, int d, float base, cudaStream_t stream);
 int gemm_error_flag(int reset);
 int exchange_error_flag(int reset);
+int few_error_flag(int reset);            // time-outs of the few-token MoE kernel
 int cache_error_flag(int reset);          // bad page ids and lengths seen by the cache-weight kernels
 size_t exchange_bytes(int world, long long rows, int d_v);
 int launch_exchange_merge(const float *O_part, const float *m_part, const float *l_part, int num_parts, void *msg,

@@ -11,12 +11,14 @@
 // rounding of a 32-bit sum would otherwise pick different experts in different kernels).
 //
 // Bound: the weights of the experts that win, 6 d f bytes each, read once for all tokens.
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <math_constants.h>
 #include <stdint.h>
 
 #include "common.cuh"
+#include "ptx.cuh"
 
 namespace fdmla {
 namespace few {
@@ -282,6 +284,8 @@ static int run_portable(const Args &a, uint8_t *ws, cudaStream_t s) {
 }  // namespace few
 }  // namespace fdmla
 
+#include "moe_few_tc.cuh"
+
 using namespace fdmla;
 
 static bool few_shape_ok(int T, int d, int f, int E, int k) {
@@ -290,8 +294,11 @@ static bool few_shape_ok(int T, int d, int f, int E, int k) {
 
 extern "C" size_t fdmla_moe_few_workspace_bytes(int T, int d, int f, int E, int k, int shared, int dtype) {
     if (T <= 0 || d <= 0 || f <= 0 || E <= 0 || k <= 0 || !few_shape_ok(T, d, f, E, k)) return 0;
-    (void)dtype;
-    return few::portable_layout(T, d, f, E, k, shared != 0).total;
+    // the larger of the two families' needs: which one runs also depends on fdmla_set_backend and on the pointers
+    const size_t simt = few::portable_layout(T, d, f, E, k, shared != 0).total;
+    if (!few::tc_supported(d, f, E, dtype)) return simt;
+    const size_t tc = few::tc_layout(T, d, f, E, k, shared != 0).total;
+    return tc > simt ? tc : simt;
 }
 
 extern "C" int fdmla_moe_few(const void *x, const float *Wg, const void *W1, const void *W3, const void *W2, const void *S1,
@@ -307,7 +314,12 @@ extern "C" int fdmla_moe_few(const void *x, const float *Wg, const void *W1, con
         workspace_bytes < fdmla_moe_few_workspace_bytes(T, d, f, E, k, shared, dtype)) return FDMLA_ERR_WORKSPACE;
     const few::Args a{x, Wg, W1, W3, W2, S1, S3, S2, out, T, d, f, E, k, shared};
     cudaStream_t s = (cudaStream_t)stream;
-    if (fdmla_get_backend() == FDMLA_BACKEND_TENSOR) return FDMLA_ERR_UNSUPPORTED;
+    const bool tc = few::tc_supported(d, f, E, dtype) && few::tc_aligned(a);
+    if (fdmla_get_backend() == FDMLA_BACKEND_TENSOR && !tc) return FDMLA_ERR_UNSUPPORTED;
+    if (tc && tensor_kernels_allowed()) {
+        note_kernel("tcgen05");
+        return few::run_tensor(a, static_cast<uint8_t *>(workspace), s);
+    }
     note_kernel("portable");
     return dtype == FDMLA_F32 ? few::run_portable<float>(a, static_cast<uint8_t *>(workspace), s)
                               : few::run_portable<__nv_bfloat16>(a, static_cast<uint8_t *>(workspace), s);
