@@ -31,24 +31,24 @@ __device__ __forceinline__ float silu(float x) { return x / (1.f + __expf(-x)); 
 // Block (32 experts, one of gridDim.y slices of d, 8 tokens): a lane owns an expert, a warp every 16th row of the slice.
 // part[s, t, e] holds slice s's share of the logit.  The widths of real gates leave a few hundred rows per block, so that
 // every warp has most of its loads in flight at once.  All blocks together also clear the counters of the kernel behind.
-constexpr int GATE_THREADS = 512, GATE_TOK = 8, GATE_ROWS = 256;
+constexpr int GATE_THREADS = 512, GATE_TOK = 8, GATE_ROWS = 256, MAX_SLICES = 32;
 
-template <typename T>
+template <typename T, int TOK>
 __global__ void __launch_bounds__(GATE_THREADS) gate_kernel(const T *__restrict__ x, const float *__restrict__ Wg,
                                                             double *__restrict__ part, unsigned *__restrict__ counters,
                                                             int n_counters, int n_tok, int d, int E) {
-    __shared__ double s_x[GATE_ROWS][GATE_TOK];                  // 16 KB; later the warps' partial sums
+    __shared__ double s_x[GATE_ROWS][TOK];                       // later the warps' partial sums
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int e = blockIdx.x * 32 + lane, t0 = blockIdx.z * GATE_TOK;
+    const int e = blockIdx.x * 32 + lane, t0 = blockIdx.z * TOK;
     {
         const int block = (blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x;
         const int blocks = gridDim.x * gridDim.y * gridDim.z;
         for (int i = block * GATE_THREADS + threadIdx.x; i < n_counters; i += blocks * GATE_THREADS) counters[i] = 0u;
     }
     const int lo = (int)((long long)d * blockIdx.y / gridDim.y), hi = (int)((long long)d * (blockIdx.y + 1) / gridDim.y);
-    double acc[GATE_TOK];
+    double acc[TOK];
 #pragma unroll
-    for (int j = 0; j < GATE_TOK; ++j) acc[j] = 0.0;
+    for (int j = 0; j < TOK; ++j) acc[j] = 0.0;
     for (int r0 = lo; r0 < hi; r0 += GATE_ROWS) {
         const int rows = hi - r0 < GATE_ROWS ? hi - r0 : GATE_ROWS;
         float wv[GATE_ROWS / 16];
@@ -58,7 +58,7 @@ __global__ void __launch_bounds__(GATE_THREADS) gate_kernel(const T *__restrict_
             wv[i] = (r < rows && e < E) ? __ldg(Wg + (size_t)(r0 + r) * E + e) : 0.f;
         }
         __syncthreads();
-        for (int i = threadIdx.x; i < GATE_ROWS * GATE_TOK; i += GATE_THREADS) {
+        for (int i = threadIdx.x; i < GATE_ROWS * TOK; i += GATE_THREADS) {
             const int r = i % GATE_ROWS, j = i / GATE_ROWS;
             s_x[r][j] = (r < rows && t0 + j < n_tok) ? (double)to_f32(x[(size_t)(t0 + j) * d + r0 + r]) : 0.0;
         }
@@ -69,84 +69,111 @@ __global__ void __launch_bounds__(GATE_THREADS) gate_kernel(const T *__restrict_
             if (r >= rows) break;
             const double wd = (double)wv[i];
 #pragma unroll
-            for (int j = 0; j < GATE_TOK; ++j) acc[j] = fma(s_x[r][j], wd, acc[j]);
+            for (int j = 0; j < TOK; ++j) acc[j] = fma(s_x[r][j], wd, acc[j]);
         }
     }
-    // the warps' sums, half of the warps at a time through the staging buffer: [8 warps][32 lanes][8 tokens]
+    // the warps' sums, half of the warps at a time through the staging buffer: [8 warps][tokens][32 lanes]
     double *red = &s_x[0][0];
     for (int step = 8; step > 0; step >>= 1) {
         __syncthreads();
         if (warp >= step && warp < 2 * step) {
 #pragma unroll
-            for (int j = 0; j < GATE_TOK; ++j) red[((warp - step) * GATE_TOK + j) * 32 + lane] = acc[j];
+            for (int j = 0; j < TOK; ++j) red[((warp - step) * TOK + j) * 32 + lane] = acc[j];
         }
         __syncthreads();
         if (warp < step) {
 #pragma unroll
-            for (int j = 0; j < GATE_TOK; ++j) acc[j] += red[(warp * GATE_TOK + j) * 32 + lane];
+            for (int j = 0; j < TOK; ++j) acc[j] += red[(warp * TOK + j) * 32 + lane];
         }
     }
     if (warp == 0 && e < E) {
 #pragma unroll
-        for (int j = 0; j < GATE_TOK; ++j)
+        for (int j = 0; j < TOK; ++j)
             if (t0 + j < n_tok) part[((size_t)blockIdx.y * n_tok + t0 + j) * E + e] = acc[j];
     }
+}
+
+template <typename T>
+static int launch_gate(const void *x, const float *Wg, double *part, unsigned *counters, int n_counters, int n_tok, int d, int E,
+                       int slices, cudaStream_t s) {
+    const dim3 grid((E + 31) / 32, slices, (n_tok + GATE_TOK - 1) / GATE_TOK);
+    if (n_tok == 1) gate_kernel<T, 1><<<grid, GATE_THREADS, 0, s>>>(static_cast<const T *>(x), Wg, part, counters, n_counters, n_tok, d, E);
+    else gate_kernel<T, GATE_TOK><<<grid, GATE_THREADS, 0, s>>>(static_cast<const T *>(x), Wg, part, counters, n_counters, n_tok, d, E);
+    return check_launch();
 }
 
 // slices of d: enough blocks for every SM, at least 64 rows each
 static int gate_slices(int n_tok, int d, int E) {
     const int blocks = ((E + 31) / 32) * ((n_tok + GATE_TOK - 1) / GATE_TOK);
     int s = (2 * kNumSMs + blocks - 1) / blocks;
-    if (s > 16) s = 16;
+    if (s > MAX_SLICES) s = MAX_SLICES;
     if (s > d / 64) s = d / 64;
     return s < 1 ? 1 : s;
 }
 
-// The k winners of one token by one warp; z [E] are its logits in shared memory.  A NaN logit never wins (so every index is
-// an expert) but makes the token's weights NaN, as a softmax over the logits would.
-__device__ __forceinline__ void topk_warp(const double *z, int E, int k, int32_t *__restrict__ idx, float *__restrict__ w, int lane) {
-    unsigned long long taken = 0;               // bit s: expert lane + 32 s has won (E <= 2048)
-    bool nan = false;
-    for (int e = lane; e < E; e += 32) nan |= isnan(z[e]);
-    nan = __any_sync(0xffffffffu, nan);
+// Logits as integers of the same order; a NaN is below every number (it never wins while a number is left).  0 marks a winner.
+__device__ __forceinline__ unsigned long long logit_key(double z) {
+    const unsigned long long u = (unsigned long long)__double_as_longlong(z + 0.0);     // -0 and 0 tie
+    return isnan(z) ? 1ull : ((u >> 63) ? ~u : (u | (1ull << 63)));
+}
+__device__ __forceinline__ double key_logit(unsigned long long key) {
+    return __longlong_as_double((long long)((key >> 63) ? (key & ~(1ull << 63)) : ~key));
+}
+
+// The k winners of one token by one warp; key [E] (shared memory) is overwritten.  `nan`: some logit of the token is NaN, and
+// so are its weights then, as those of a softmax over the logits would be.  Every lane keeps the best of its experts, a round
+// is three warp reductions (high half, low half, index) and a new scan by the lane that lost its best.
+__device__ __forceinline__ void topk_warp(unsigned long long *key, int E, int k, bool nan, int32_t *__restrict__ idx,
+                                          float *__restrict__ w, int lane) {
+    unsigned long long best = 0;
+    int at = 0x7fffffff;
+    auto scan = [&]() {
+        best = 0;
+        at = 0x7fffffff;
+        for (int e = lane; e < E; e += 32)
+            if (key[e] > best) { best = key[e]; at = e; }
+    };
+    scan();
     double z0 = 0.0;
     float my_w = 0.f, sum = 0.f;
     int my_i = 0;
     for (int j = 0; j < k; ++j) {
-        double bv = -CUDART_INF;
-        int bi = 0x7fffffff;
-        for (int e = lane, s = 0; e < E; e += 32, ++s) {
-            if ((taken >> s) & 1ull) continue;
-            const double v = isnan(z[e]) ? -CUDART_INF : z[e];
-            if (v > bv || bi == 0x7fffffff) { bv = v; bi = e; }
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const double ov = __shfl_xor_sync(0xffffffffu, bv, o);
-            const int oi = __shfl_xor_sync(0xffffffffu, bi, o);
-            if (oi != 0x7fffffff && (bi == 0x7fffffff || ov > bv || (ov == bv && oi < bi))) { bv = ov; bi = oi; }
-        }
-        if ((bi & 31) == lane) taken |= 1ull << (bi >> 5);
-        if (j == 0) z0 = bv;
-        const float pj = nan ? CUDART_NAN_F : expf((float)(bv - z0));
+        const uint32_t hi = (uint32_t)(best >> 32), top = __reduce_max_sync(0xffffffffu, hi);
+        const uint32_t lo = hi == top ? (uint32_t)best : 0u, low = __reduce_max_sync(0xffffffffu, lo);
+        const int i = (int)__reduce_min_sync(0xffffffffu, hi == top && (uint32_t)best == low ? (uint32_t)at : 0x7fffffffu);
+        const double z = key_logit(((unsigned long long)top << 32) | low);
+        if (at == i) { key[i] = 0ull; scan(); }
+        if (j == 0) z0 = z;
+        const float pj = nan ? CUDART_NAN_F : expf((float)(z - z0));
         sum += pj;
-        if (lane == j) { my_w = pj; my_i = bi; }
+        if (lane == j) { my_w = pj; my_i = i; }
     }
     if (lane < k) { idx[lane] = my_i; w[lane] = my_w / sum; }
+}
+
+// Sum of a logit's slices, in order, all loads in flight.
+__device__ __forceinline__ double logit(const double *__restrict__ part, int slices, size_t stride) {
+    double v[MAX_SLICES], z = 0.0;
+#pragma unroll
+    for (int s = 0; s < MAX_SLICES; ++s) v[s] = s < slices ? part[(size_t)s * stride] : 0.0;
+#pragma unroll
+    for (int s = 0; s < MAX_SLICES; ++s) z += v[s];
+    return z;
 }
 
 // ---- the layer on CUDA cores: any type, any width ------------------------------------------------------------------------
 __global__ void __launch_bounds__(128) route_kernel(const double *__restrict__ part, int slices, int32_t *__restrict__ idx,
                                                     float *__restrict__ w, int n_tok, int E, int k) {
-    extern __shared__ double s_z[];
+    extern __shared__ unsigned long long s_key[];
     const int t = blockIdx.x;
+    bool nan = false;
     for (int e = threadIdx.x; e < E; e += blockDim.x) {
-        double v = 0.0;
-        for (int s = 0; s < slices; ++s) v += part[((size_t)s * n_tok + t) * E + e];
-        s_z[e] = v;
+        const double z = logit(part + (size_t)t * E + e, slices, (size_t)n_tok * E);
+        s_key[e] = logit_key(z);
+        nan |= isnan(z);
     }
-    __syncthreads();
-    if (threadIdx.x < 32) topk_warp(s_z, E, k, idx + (size_t)t * k, w + (size_t)t * k, threadIdx.x);
+    nan = __syncthreads_or(nan);
+    if (threadIdx.x < 32) topk_warp(s_key, E, k, nan, idx + (size_t)t * k, w + (size_t)t * k, threadIdx.x);
 }
 
 // Tokens (and the slots j of their choices) of expert e, in token order; expert E is the shared one (every token).
@@ -269,8 +296,7 @@ static int run_portable(const Args &a, uint8_t *ws, cudaStream_t s) {
     int32_t *idx = reinterpret_cast<int32_t *>(ws + L.idx);
     float *w = reinterpret_cast<float *>(ws + L.w), *h = reinterpret_cast<float *>(ws + L.h), *y = reinterpret_cast<float *>(ws + L.y);
     const int slices = gate_slices(a.n_tok, a.d, a.E);
-    gate_kernel<T><<<dim3((a.E + 31) / 32, slices, (a.n_tok + GATE_TOK - 1) / GATE_TOK), GATE_THREADS, 0, s>>>(
-        static_cast<const T *>(a.x), a.Wg, part, nullptr, 0, a.n_tok, a.d, a.E);
+    if (launch_gate<T>(a.x, a.Wg, part, nullptr, 0, a.n_tok, a.d, a.E, slices, s) != FDMLA_OK) return FDMLA_ERR_CUDA;
     route_kernel<<<a.n_tok, 128, a.E * sizeof(double), s>>>(part, slices, idx, w, a.n_tok, a.E, a.k);
     expert_kernel<T, T, true><<<dim3((a.f + SIMT_COLS - 1) / SIMT_COLS, a.E + a.shared), 256, 0, s>>>(
         static_cast<const T *>(a.x), static_cast<const T *>(a.W1), static_cast<const T *>(a.W3), static_cast<const T *>(a.S1),

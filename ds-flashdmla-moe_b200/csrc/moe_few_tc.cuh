@@ -1,22 +1,25 @@
 // The MoE layer for few tokens on the tensor cores: one persistent kernel behind the gate kernel (included by moe_few.cu).
 //
 // Everything is bound by reading the weights of the experts that won, so the weights are the M side of the products (128
-// weight columns per tile) and ALL tokens of the call the N side (16 .. 128 columns): an expert's weights pass through shared
-// memory once, whatever the number of its tokens, and a token that did not choose the expert costs a column of zeros, not a
-// gather.
-//   stage 1   D1 = W1_e^T x^T, D3 = W3_e^T x^T; h[e, t] = gate[t, e] silu(D1) D3, 0 for tokens that did not choose e
-//   stage 2   out^T = sum_e W2_e^T h_e^T: one accumulator for all experts of the call (the shared expert is one more with gate
-//             weight 1), so there is no scatter, no combine pass and one rounding of the result.  h carries the gate weight and
-//             is rounded to bf16 for the tensor cores: a relative error of at most 2^-8 per element, as without the weight.
+// weight columns per tile) and the tokens the N side: an expert's weights pass through shared memory once, whatever the number
+// of its tokens.
+//   stage 1   D1 = W1_e^T x^T, D3 = W3_e^T x^T for all tokens of the call (16 .. 128 columns; no gather), of which the columns of
+//             the tokens that chose e give rows of h = silu(D1) D3, rounded to bf16 for the tensor cores
+//   stage 2   y^T = W2_e^T h_e^T over e's rows of h (groups of at most 64)
+//   stage 3   out[t] = sum over t's choices of w y, plus the shared expert's y, rounded once
 //
-// The work of either stage is cut into equal contiguous runs of 64-deep steps, one run per CTA; a tile that two or more CTAs
-// share is left as fp32 pieces in scratch and summed, piece by piece in order, by the CTA that finishes last (tickets; the
-// result does not depend on who that is).  Grid barriers (cooperative launch: all CTAs are resident) stand behind the top-k and
-// between the stages; the producer warp fills its ring with stage 2's weights before the second barrier, so HBM does not idle.
+// Work is handed out in items, in the order in which they lie in memory (neighbouring CTAs read neighbouring columns of the same
+// rows): the first by CTA number, the rest from a counter, because CTAs that read the same number of bytes finish up to a
+// quarter apart.  A tile is cut along its reduction into `split` items when there are few tiles; the fp32 pieces are summed in order
+// behind the next barrier, by all CTAs.  Grid barriers (cooperative launch: all CTAs are resident) stand behind the top-k and
+// between the stages; ahead of stage 2 the producer warp fills its ring with weights and has the next ones brought into L2, so
+// HBM does not idle.
 //
 // Warp 0 issues the copies, warp 1 the MMAs, warps 2-5 read the accumulators (thread = weight column).  All waits are bounded
 // (codes 41-44 of fdmla_device_error_flag).
 #pragma once
+
+#include <type_traits>
 
 namespace fdmla {
 
@@ -31,51 +34,64 @@ constexpr int MAX_E = 2048;
 enum { ERR_PRODUCER = 41, ERR_MMA = 42, ERR_EPILOGUE = 43, ERR_GRID = 44 };
 __device__ int g_few_error = 0;
 
-// NP: tokens of the call rounded up to the width of the MMA's N side.  The ring takes what shared memory has left: 196 to
-// 216 KB; about 50 KB in flight per SM cover the latency of HBM at full bandwidth.
+// NP: tokens of the call rounded up to the width of the MMA's N side in stage 1.  The ring takes 180 to 200 KB of shared memory;
+// about 50 KB in flight per SM cover the latency of HBM at full bandwidth.
+constexpr int GROUP = 64;                             // rows of h in one accumulator of stage 2
 template <int NP> struct Cfg {
-    static constexpr int B_STEP = NP * 128;           // 64 activations of every token
-    static constexpr int STAGE = A_BYTES + 2 * B_STEP;
-    static constexpr int STAGES = NP == 16 ? 6 : (NP == 32 ? 5 : (NP == 64 ? 4 : 3));
+    static constexpr int GN = NP < GROUP ? NP : GROUP;
+    static constexpr int B_BYTES = (NP > 2 * GN ? NP : 2 * GN) * 128;   // 64 activations of all tokens / 2 x 64 of a group
+    static constexpr int STAGE = A_BYTES + B_BYTES;
+    static constexpr int STAGES = NP <= 32 ? 5 : 4;
     static constexpr int COLS = 4 * NP;               // tensor memory: two buffers of (D1, D3)
-    static constexpr int SMEM = 1024 + STAGES * STAGE + 6144;
+    static constexpr int SMEM = 1024 + STAGES * STAGE + 25600;
     static_assert(SMEM <= kMaxSmemPerBlock, "shared memory overflow");
 };
+constexpr int MAX_ROWS = MAX_T * 32, MAX_GROUPS = MAX_E + 2 + MAX_ROWS / GROUP;
+constexpr int QUEUE = 16;                             // items under way: at most 5 ring stages + 2 accumulators + 2
+constexpr unsigned NO_ITEM = 0xffffffffu;
+constexpr int N_COUNTERS = 6;
 
 struct TcShared {                                     // behind the ring
-    uint64_t bars[2 * 6 + 4];
-    uint32_t tmem, bitmap[MAX_E / 32];
-    int n_active, last, dead;
-    float gate[MAX_T];
-    uint16_t list[MAX_E];
+    uint64_t bars[2 * 5 + 4 + QUEUE];
+    uint32_t tmem, queue[QUEUE], ahead[5], scan[16];
+    int n_routed, n_groups, last, dead;
+    uint16_t expert[MAX_E];                           // routed experts, ascending
+    uint16_t first[MAX_E + 1];                        // their first rows of h
+    uint16_t group[MAX_GROUPS];                       // routed expert (or n_routed: the shared one) | second group << 15
+    uint8_t token[MAX_ROWS];                          // of every row of h
+    uint16_t row[MAX_ROWS];                           // of every choice (t, j)
 };
-static_assert(sizeof(TcShared) <= 6144, "TcShared outgrew its space");
+static_assert(sizeof(TcShared) <= 25600, "TcShared outgrew its space");
 
 struct TcProblem {
     int n_tok, d, f, E, k, shared, slices;
     int ft, kc1, nt, fs;                              // 128-wide tiles of f, 64-deep steps of d, 128-wide tiles of d, 128-deep pairs of steps of f
+    int split_cap, rows;                              // most items per tile that the scratch holds; rows of h
     const double *part;
     int32_t *idx;
     float *w;
-    unsigned *bars, *tickets1, *tickets2;             // zero at launch
-    __nv_bfloat16 *h;                                 // [active expert, token, f]
-    float *pieces;                                    // [2 per CTA][2 n_tok][128]
+    unsigned *bars, *next;                            // [4] grid barriers, [2] item counters: zero at launch
+    __nv_bfloat16 *h;                                 // [rows, f], the shared expert's rows last
+    float *pieces;                                    // stage 1: [split][rows][2][ft 128]; stage 2: y [split][rows][d]
     __nv_bfloat16 *out;
 };
 
-// One stage's work: `per` units (ring stages) a tile, units 0 .. total - 1 dealt out in contiguous runs to the first `ctas` CTAs.
-struct Runs {
-    unsigned total, per, ctas;
-    __device__ __forceinline__ Runs(unsigned tiles, unsigned per_, unsigned grid) : total(tiles * per_), per(per_), ctas(grid < total ? grid : total) {}
-    __device__ __forceinline__ unsigned start(unsigned c) const { return c >= ctas ? total : (unsigned)((unsigned long long)total * c / ctas); }
-    __device__ __forceinline__ unsigned owner(unsigned u) const { return (unsigned)((((unsigned long long)u + 1) * ctas - 1) / total); }
+// Items of a stage: tiles x split, `per` units (ring stages) a tile.  About a dozen items per CTA even out the CTAs' speeds; an
+// item has two units at least.
+struct Items {
+    unsigned per, split, total;
+    __device__ __forceinline__ Items(unsigned tiles, unsigned per_, unsigned cap) : per(per_) {
+        unsigned s = (12 * gridDim.x + tiles - 1) / tiles;
+        s = min(min(s, cap), per / 2);
+        split = max(s, 1u);
+        total = tiles * split;
+    }
+    __device__ __forceinline__ unsigned begin(unsigned s) const { return per * s / split; }
 };
 
 __device__ __forceinline__ bool grid_wait(const unsigned *bar, unsigned n) {
-    for (uint32_t it = 0; it < (16u << 20); ++it) {
+    for (uint32_t it = 0; it < (8u << 20); ++it)
         if (ptx::ld_acquire_gpu(bar) >= n) return true;
-        __nanosleep(32);
-    }
     return false;
 }
 
@@ -86,7 +102,7 @@ layer_kernel(const TcProblem p, const __grid_constant__ CUtensorMap tmX, const _
              const __grid_constant__ CUtensorMap tmS1, const __grid_constant__ CUtensorMap tmS3, const __grid_constant__ CUtensorMap tmS2) {
     using namespace ptx;
     using C = Cfg<NP>;
-    constexpr int STAGES = C::STAGES, STAGE = C::STAGE, B_STEP = C::B_STEP;
+    constexpr int STAGES = C::STAGES, STAGE = C::STAGE;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *ring = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     TcShared &sh = *reinterpret_cast<TcShared *>(ring + STAGES * STAGE);
@@ -95,31 +111,37 @@ layer_kernel(const TcProblem p, const __grid_constant__ CUtensorMap tmX, const _
     auto EMPTY = [&](int s) { return bar0 + 8u * (STAGES + s); };
     auto ACC_FULL = [&](int a) { return bar0 + 8u * (2 * STAGES + a); };
     auto ACC_EMPTY = [&](int a) { return bar0 + 8u * (2 * STAGES + 2 + a); };
+    auto QUEUED = [&](int q) { return bar0 + 8u * (2 * STAGES + 4 + q); };
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int choices = p.n_tok * p.k;
 
     if (tid == 0) {
         sh.dead = *reinterpret_cast<volatile int *>(&g_few_error) != 0;      // an earlier launch gave up a wait: do nothing
         for (int s = 0; s < STAGES; ++s) { mbar_init(FULL(s), 1); mbar_init(EMPTY(s), 1); }
         for (int a = 0; a < 2; ++a) { mbar_init(ACC_FULL(a), 1); mbar_init(ACC_EMPTY(a), 128); }
+        for (int q = 0; q < QUEUE; ++q) mbar_init(QUEUED(q), 1);
+        sh.last = 0;
         fence_mbar_init();
     }
     if (warp == 1) { tmem_alloc(smem_u32(&sh.tmem), C::COLS); tmem_relinquish(); }
-    for (int i = tid; i < MAX_E / 32; i += TC_THREADS) sh.bitmap[i] = 0u;
 
-    // ---- top-k: one token per CTA; the slices of its logits are summed in order, in shared memory that the ring uses later ----
-    double *s_z = reinterpret_cast<double *>(ring);
+    // ---- top-k: one token per CTA, in shared memory that the ring uses later ---------------------------------------------------
+    unsigned long long *s_key = reinterpret_cast<unsigned long long *>(ring);
     for (int t = blockIdx.x; t < p.n_tok; t += gridDim.x) {
+        bool nan = false;
         for (int e = tid; e < p.E; e += TC_THREADS) {
-            double v = 0.0;
-            for (int s = 0; s < p.slices; ++s) v += p.part[((size_t)s * p.n_tok + t) * p.E + e];
-            s_z[e] = v;
+            const double z = logit(p.part + (size_t)t * p.E + e, p.slices, (size_t)p.n_tok * p.E);
+            s_key[e] = logit_key(z);
+            nan |= isnan(z);
         }
-        __syncthreads();
-        if (warp == 0) topk_warp(s_z, p.E, p.k, p.idx + (size_t)t * p.k, p.w + (size_t)t * p.k, lane);
+        nan = __syncthreads_or(nan);
+        if (warp == 0) topk_warp(s_key, p.E, p.k, nan, p.idx + (size_t)t * p.k, p.w + (size_t)t * p.k, lane);
         __syncthreads();
     }
-    fence_proxy_async_all();
-    __syncthreads();
+    // which tokens chose an expert: a 128-bit mask each
+    uint32_t(*s_mask)[4] = reinterpret_cast<uint32_t(*)[4]>(ring + 16384);
+    uint16_t *s_first = reinterpret_cast<uint16_t *>(ring + 16384 + MAX_E * 16);
+    for (int i = tid; i < p.E * 4; i += TC_THREADS) (&s_mask[0][0])[i] = 0u;
     if (tid == 0 && !sh.dead) {
         __threadfence();
         atomicAdd(p.bars, 1u);
@@ -130,115 +152,229 @@ layer_kernel(const TcProblem p, const __grid_constant__ CUtensorMap tmX, const _
     tc_fence_after_sync();
     const uint32_t tmem = sh.tmem;
     const bool dead = sh.dead != 0;
-    // ---- the experts that won, ascending; the shared one is the last ---------------------------------------------------------
+    // ---- routed experts in ascending order, their rows of h in token order (the same in every CTA) -------------------------------
     if (!dead)
-        for (int i = tid; i < p.n_tok * p.k; i += TC_THREADS) {
-            const int e = __ldcg(p.idx + i);
-            atomicOr(&sh.bitmap[e >> 5], 1u << (e & 31));
+        for (int i = tid; i < choices; i += TC_THREADS) {
+            const int e = __ldcg(p.idx + i), t = i / p.k;
+            atomicOr(&s_mask[e][t >> 5], 1u << (t & 31));
         }
     __syncthreads();
-    if (warp == 0) {
-        uint32_t b0 = sh.bitmap[2 * lane], b1 = sh.bitmap[2 * lane + 1];
-        const int n = __popc(b0) + __popc(b1);
-        int at = n;
+    {   // a thread owns `per` neighbouring experts; prefix sums of (experts, groups) and rows over the block
+        const int per = (p.E + TC_THREADS - 1) / TC_THREADS, e0 = min(tid * per, p.E), e1 = min(e0 + per, p.E);
+        auto tokens = [&](int e) { return __popc(s_mask[e][0]) + __popc(s_mask[e][1]) + __popc(s_mask[e][2]) + __popc(s_mask[e][3]); };
+        uint32_t cnt = 0, rows = 0;                    // experts | groups << 16
+        for (int e = e0; e < e1; ++e) {
+            const int n = tokens(e);
+            cnt += (n > 0 ? 0x10001u : 0u) + (n > GROUP ? 0x10000u : 0u);
+            rows += n;
+        }
+        uint32_t ci = cnt, ri = rows;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int u = __shfl_up_sync(0xffffffffu, at, o);
-            if (lane >= o) at += u;
+            const uint32_t cu = __shfl_up_sync(0xffffffffu, ci, o), ru = __shfl_up_sync(0xffffffffu, ri, o);
+            if (lane >= o) { ci += cu; ri += ru; }
         }
-        if (lane == 31) sh.n_active = at;
-        at -= n;
-        for (; b0; b0 &= b0 - 1) sh.list[at++] = (uint16_t)(64 * lane + __ffs(b0) - 1);
-        for (; b1; b1 &= b1 - 1) sh.list[at++] = (uint16_t)(64 * lane + 32 + __ffs(b1) - 1);
+        if (lane == 31) { sh.scan[warp] = ci; sh.scan[8 + warp] = ri; }
+        __syncthreads();
+        for (int v = 0; v < warp; ++v) { ci += sh.scan[v]; ri += sh.scan[8 + v]; }
+        uint32_t c = ci - cnt, r = ri - rows;
+        for (int e = e0; e < e1; ++e) {
+            const int n = tokens(e);
+            if (n == 0) continue;
+            const uint32_t a = c & 0xffffu, g = c >> 16;
+            sh.expert[a] = (uint16_t)e;
+            sh.first[a] = s_first[e] = (uint16_t)r;
+            sh.group[g] = (uint16_t)a;
+            if (n > GROUP) sh.group[g + 1] = (uint16_t)(a | 0x8000);
+            c += 0x10001u + (n > GROUP ? 0x10000u : 0u);
+            r += n;
+        }
+        if (tid == TC_THREADS - 1) {
+            int n_grp = ci >> 16;
+            sh.n_routed = ci & 0xffffu;
+            sh.first[sh.n_routed] = (uint16_t)ri;
+            if (p.shared) {
+                sh.group[n_grp++] = (uint16_t)sh.n_routed;
+                if (p.n_tok > GROUP) sh.group[n_grp++] = (uint16_t)(sh.n_routed | 0x8000);
+            }
+            sh.n_groups = n_grp;
+        }
     }
     __syncthreads();
-    const unsigned routed = sh.n_active, active = routed + p.shared;
-    const Runs r1(active * p.ft, p.kc1, gridDim.x), r2(p.nt, active * p.fs, gridDim.x);
-    const unsigned cta = blockIdx.x;
-    const unsigned u1_lo = dead ? 0 : r1.start(cta), u1_hi = dead ? 0 : r1.start(cta + 1);
-    const unsigned u2_lo = dead ? 0 : r2.start(cta), u2_hi = dead ? 0 : r2.start(cta + 1);
+    if (!dead)
+        for (int i = tid; i < choices; i += TC_THREADS) {
+            const int e = __ldcg(p.idx + i), t = i / p.k;
+            int r = s_first[e];
+            for (int q = 0; q < t >> 5; ++q) r += __popc(s_mask[e][q]);
+            r += __popc(s_mask[e][t >> 5] & ((1u << (t & 31)) - 1u));
+            sh.row[i] = (uint16_t)r;
+            sh.token[r] = (uint8_t)t;
+        }
+    fence_proxy_async_all();                           // the copies write where the masks were
+    __syncthreads();
+    const unsigned routed = sh.n_routed;
+    const Items it1(max((routed + p.shared) * p.ft, 1u), p.kc1, p.split_cap), it2(max(sh.n_groups * p.nt, 1), p.fs, p.split_cap);
     const int f_steps = p.f / 64;
+    // rows of h of routed expert a (a == routed: the shared expert), and of group g
+    auto rows_of = [&](unsigned a, int &row0) {
+        row0 = a < routed ? (int)sh.first[a] : choices;
+        return (a < routed ? (int)sh.first[a + 1] : choices + p.n_tok) - row0;
+    };
+    auto group_of = [&](unsigned g, unsigned &a, int &row0) {
+        a = sh.group[g] & 0x7fff;
+        const int skip = sh.group[g] >> 15 ? GROUP : 0, n = rows_of(a, row0) - skip;
+        row0 += skip;
+        return min(n, GROUP);
+    };
 
     if (warp == 0) {
         // ================================ producer ================================
         const bool elected = elect_one();
         if (lane == 0) { prefetch_tmap(&tmX); prefetch_tmap(&tmW1); prefetch_tmap(&tmW3); prefetch_tmap(&tmW2); prefetch_tmap(&tmH); }
         bool ok = !dead;
-        int s = 0, use = 0;
-        for (unsigned u = u1_lo; u < u1_hi && ok;) {
-            const unsigned tile = u / r1.per, a = tile / p.ft, i = tile - a * p.ft, k0 = u - tile * r1.per;
-            const unsigned k1 = min(r1.per, k0 + (u1_hi - u));
+        int s = 0, use = 0, n_items = 0;
+        // the next item is asked for while the current one is loaded; the counter's first answer is item gridDim.x
+        auto ask = [&](int stage, unsigned taken) { return lane == 0 ? taken + atomicAdd(p.next + stage - 1, 1u) : 0u; };
+        auto announce = [&](unsigned item) {
+            if (lane == 0) {
+                sh.queue[n_items % QUEUE] = item;
+                mbar_arrive(QUEUED(n_items % QUEUE));
+            }
+            ++n_items;
+        };
+        unsigned ans = 0;
+        for (unsigned item = blockIdx.x; ok && item < it1.total; item = __shfl_sync(0xffffffffu, ans, 0)) {
+            ans = ask(1, gridDim.x);
+            announce(item);
+            const unsigned i = item % p.ft, q = item / p.ft, a = q / it1.split, ks = q - a * it1.split;
             const bool own = a >= routed;
             const CUtensorMap *m1 = own ? &tmS1 : &tmW1, *m3 = own ? &tmS3 : &tmW3;
-            const int row0 = own ? 0 : (int)sh.list[a] * p.d;
-            for (unsigned kc = k0; kc < k1 && ok; ++kc) {
+            const int row0 = own ? 0 : (int)sh.expert[a] * p.d;
+            for (unsigned kc = it1.begin(ks); kc < it1.begin(ks + 1) && ok; ++kc) {
                 if (use > 0) ok = mbar_wait(EMPTY(s), (use - 1) & 1);
                 if (ok && elected) {
                     const uint32_t dst = smem_u32(ring + s * STAGE);
-                    mbar_arrive_expect_tx(FULL(s), A_BYTES + B_STEP);
+                    mbar_arrive_expect_tx(FULL(s), A_BYTES + NP * 128);
                     tma_load_3d(dst, m1, 0, row0 + (int)kc * 64, (int)i * 2, FULL(s));
                     tma_load_3d(dst + A_BYTES / 2, m3, 0, row0 + (int)kc * 64, (int)i * 2, FULL(s));
                     tma_load_2d(dst + A_BYTES, &tmX, (int)kc * 64, 0, FULL(s));
                 }
                 if (++s == STAGES) { s = 0; ++use; }
             }
-            u += k1 - k0;
         }
-        // stage 2: weights of the first units ahead of the barrier, the activations h behind it
-        auto load = [&](unsigned u, int slot, bool weights, bool acts) {
-            const unsigned j = u / r2.per, q = u - j * r2.per, a = q / p.fs, c2 = q - a * p.fs;
+        announce(NO_ITEM);
+        // stage 2: weights of the first units ahead of the barrier, their rows of h behind it
+        auto weights = [&](unsigned a, unsigned j, unsigned c2, int n16, int slot) {
             const bool own = a >= routed;
-            const int row0 = (own ? 0 : (int)sh.list[a] * p.f) + (int)c2 * 128;
-            const int nk = min(2, f_steps - 2 * (int)c2);
+            const int row0 = (own ? 0 : (int)sh.expert[a] * p.f) + (int)c2 * 128, nk = min(2, f_steps - 2 * (int)c2);
             const uint32_t dst = smem_u32(ring + slot * STAGE);
-            if (weights) {
-                mbar_arrive_expect_tx(FULL(slot), nk * (A_BYTES / 2 + B_STEP));
-                for (int c = 0; c < nk; ++c)
-                    tma_load_3d(dst + c * (A_BYTES / 2), own ? &tmS2 : &tmW2, 0, row0 + c * 64, (int)j * 2, FULL(slot));
-            }
-            if (acts)
-                for (int c = 0; c < nk; ++c)
-                    tma_load_2d(dst + A_BYTES + c * B_STEP, &tmH, (int)c2 * 128 + c * 64, (int)a * p.n_tok, FULL(slot));
+            mbar_arrive_expect_tx(FULL(slot), nk * (A_BYTES / 2 + n16 * 2048));
+            for (int c = 0; c < nk; ++c)
+                tma_load_3d(dst + c * (A_BYTES / 2), own ? &tmS2 : &tmW2, 0, row0 + c * 64, (int)j * 2, FULL(slot));
         };
-        const unsigned ahead = min(u2_hi - u2_lo, (unsigned)STAGES);
-        const int s_first = s;
-        for (unsigned i = 0; i < ahead && ok; ++i) {
-            if (use > 0) ok = mbar_wait(EMPTY(s), (use - 1) & 1);
-            if (ok && elected) load(u2_lo + i, s, true, false);
-            if (++s == STAGES) { s = 0; ++use; }
+        auto acts = [&](int row0, unsigned c2, int n16, int slot) {
+            const uint32_t dst = smem_u32(ring + slot * STAGE) + A_BYTES;
+            const int nk = min(2, f_steps - 2 * (int)c2);
+            for (int c = 0; c < nk; ++c)
+                for (int r = 0; r < n16; ++r)
+                    tma_load_2d(dst + (c * n16 + r) * 2048, &tmH, (int)c2 * 128 + c * 64, row0 + 16 * r, FULL(slot));
+        };
+        int n_ahead = 0;
+        bool open = false;                             // the barrier has been passed
+        auto pass = [&]() {
+            if (!grid_wait(p.bars + (it1.split > 1 ? 3 : 1), gridDim.x)) { ok = false; if (lane == 0 && !dead) atomicCAS(&g_few_error, 0, ERR_GRID); }
+            ok = __all_sync(0xffffffffu, ok);
+            fence_proxy_async_all();                   // h was written with ordinary stores
+            if (ok && elected)
+                for (int i = 0; i < n_ahead; ++i) {
+                    const uint32_t v = sh.ahead[i];    // the i-th unit ahead: group | step << 12 | ring slot << 28
+                    unsigned a;
+                    int row0;
+                    const int n = group_of(v & 0xfff, a, row0);
+                    acts(row0, (v >> 12) & 0xffff, (n + 15) >> 4, v >> 28);
+                }
+            open = true;
+        };
+        // the first items go by CTA number, so that each CTA knows which weights to have brought into L2: about 12 units
+        const unsigned fixed = min(max(it2.total / (4 * gridDim.x), 1u), (12 + it2.per / it2.split - 1) / max(it2.per / it2.split, 1u));
+        unsigned round = 0;
+        auto prefetch = [&](unsigned item, unsigned skip) {
+            const unsigned j = item % p.nt, q = item / p.nt, g = q / it2.split, ks = q - g * it2.split;
+            unsigned a;
+            int row0;
+            group_of(g, a, row0);
+            const bool own = a >= routed;
+            for (unsigned c2 = it2.begin(ks) + skip; c2 < it2.begin(ks + 1); ++c2) {
+                const int row = (own ? 0 : (int)sh.expert[a] * p.f) + (int)c2 * 128, nk = min(2, f_steps - 2 * (int)c2);
+                for (int c = 0; c < nk; ++c) tma_prefetch_3d(own ? &tmS2 : &tmW2, 0, row + c * 64, (int)j * 2);
+            }
+        };
+        for (unsigned item = blockIdx.x; ok && item < it2.total;) {
+            const bool by_number = ++round < fixed;
+            if (!by_number) ans = ask(2, fixed * gridDim.x);
+            announce(item);
+            const unsigned j = item % p.nt, q = item / p.nt, g = q / it2.split, ks = q - g * it2.split;
+            unsigned a;
+            int row0;
+            const int n16 = (group_of(g, a, row0) + 15) >> 4;
+            for (unsigned c2 = it2.begin(ks); c2 < it2.begin(ks + 1) && ok; ++c2) {
+                if (!open && n_ahead == STAGES) {
+                    if (elected) {
+                        prefetch(item, c2 - it2.begin(ks));
+                        for (unsigned r = round; r < fixed && blockIdx.x + r * gridDim.x < it2.total; ++r) prefetch(blockIdx.x + r * gridDim.x, 0);
+                    }
+                    __syncwarp();
+                    pass();
+                }
+                if (ok && use > 0) ok = mbar_wait(EMPTY(s), (use - 1) & 1);
+                if (ok && elected) {
+                    weights(a, j, c2, n16, s);
+                    if (open) acts(row0, c2, n16, s);
+                    else sh.ahead[n_ahead] = g | (c2 << 12) | ((uint32_t)s << 28);
+                }
+                if (!open) ++n_ahead;
+                if (++s == STAGES) { s = 0; ++use; }
+            }
+            item = by_number ? blockIdx.x + round * gridDim.x : __shfl_sync(0xffffffffu, ans, 0);
         }
-        if (ok && !grid_wait(p.bars + 1, gridDim.x)) { ok = false; if (lane == 0) atomicCAS(&g_few_error, 0, ERR_GRID); }
-        ok = __all_sync(0xffffffffu, ok);
-        fence_proxy_async_all();                       // h was written with ordinary stores
-        if (ok && elected)
-            for (unsigned i = 0; i < ahead; ++i) load(u2_lo + i, (s_first + (int)i) % STAGES, false, true);
-        for (unsigned u = u2_lo + ahead; u < u2_hi && ok; ++u) {
-            ok = mbar_wait(EMPTY(s), (use - 1) & 1);
-            if (ok && elected) load(u, s, true, true);
-            if (++s == STAGES) { s = 0; ++use; }
-        }
+        if (ok && !open) pass();
+        announce(NO_ITEM);
         if (!ok && !dead && lane == 0) atomicCAS(&g_few_error, 0, ERR_PRODUCER);
         __syncwarp();
     } else if (warp == 1) {
         // ================================ MMA issuer ================================
         const bool elected = elect_one();
-        constexpr uint32_t idesc = make_idesc_bf16(128, NP, 1, 0);
         bool ok = !dead;
-        int s = 0, n_done = 0;
+        int s = 0, n_done = 0, n_items = 0;
         uint32_t ph = 0;
 #pragma unroll 1
         for (int stage = 1; stage <= 2; ++stage) {
-            const unsigned per = stage == 1 ? r1.per : r2.per, hi = stage == 1 ? u1_hi : u2_hi;
-            for (unsigned u = stage == 1 ? u1_lo : u2_lo; u < hi;) {
+            for (;;) {
+                ok = ok && mbar_wait(QUEUED(n_items % QUEUE), (n_items / QUEUE) & 1);
                 if (!__all_sync(0xffffffffu, ok)) break;
-                const unsigned k0 = u % per, k1 = min(per, k0 + (hi - u));
+                const unsigned item = *reinterpret_cast<volatile uint32_t *>(&sh.queue[n_items % QUEUE]);
+                ++n_items;
+                if (item == NO_ITEM) break;
+                unsigned lo, hi;
+                int n16 = NP / 16;
+                if (stage == 1) {
+                    const unsigned ks = item / p.ft % it1.split;
+                    lo = it1.begin(ks); hi = it1.begin(ks + 1);
+                } else {
+                    const unsigned q = item / p.nt, g = q / it2.split, ks = q - g * it2.split;
+                    unsigned a;
+                    int row0;
+                    n16 = (group_of(g, a, row0) + 15) >> 4;
+                    lo = it2.begin(ks); hi = it2.begin(ks + 1);
+                }
+                const uint32_t idesc = make_idesc_bf16(128, 16 * n16, 1, 0);
                 const int acc = n_done & 1;
                 const uint32_t d0 = tmem + acc * 2 * NP;
                 if (n_done >= 2) {
                     ok = mbar_wait(ACC_EMPTY(acc), ((n_done >> 1) - 1) & 1);
                     tc_fence_after_sync();
                 }
-                for (unsigned kc = k0; kc < k1; ++kc) {
+                for (unsigned kc = lo; kc < hi; ++kc) {
                     ok = ok && mbar_wait(FULL(s), ph);
                     tc_fence_after_sync();
                     if (elected && ok) {
@@ -247,24 +383,23 @@ layer_kernel(const TcProblem p, const __grid_constant__ CUtensorMap tmX, const _
 #pragma unroll
                             for (int k = 0; k < 4; ++k) {
                                 const uint64_t db = make_smem_desc(b + k * 32, 16, 1024, kLayoutSw128);
-                                mma_bf16_ss(d0, make_smem_desc(a + k * 2048, 8192, 1024, kLayoutSw128), db, idesc, kc != k0 || k != 0);
-                                mma_bf16_ss(d0 + NP, make_smem_desc(a + A_BYTES / 2 + k * 2048, 8192, 1024, kLayoutSw128), db, idesc, kc != k0 || k != 0);
+                                mma_bf16_ss(d0, make_smem_desc(a + k * 2048, 8192, 1024, kLayoutSw128), db, idesc, kc != lo || k != 0);
+                                mma_bf16_ss(d0 + NP, make_smem_desc(a + A_BYTES / 2 + k * 2048, 8192, 1024, kLayoutSw128), db, idesc, kc != lo || k != 0);
                             }
                         } else {
-                            const int steps = min(2, f_steps - 2 * (int)(kc % p.fs));
+                            const int steps = min(2, f_steps - 2 * (int)kc);
                             for (int c = 0; c < steps; ++c)
 #pragma unroll
                                 for (int k = 0; k < 4; ++k)
                                     mma_bf16_ss(d0, make_smem_desc(a + c * (A_BYTES / 2) + k * 2048, 8192, 1024, kLayoutSw128),
-                                                make_smem_desc(b + c * B_STEP + k * 32, 16, 1024, kLayoutSw128), idesc, kc != k0 || c != 0 || k != 0);
+                                                make_smem_desc(b + c * n16 * 2048 + k * 32, 16, 1024, kLayoutSw128), idesc, kc != lo || c != 0 || k != 0);
                         }
                         mma_commit(EMPTY(s));
-                        if (kc == k1 - 1) mma_commit(ACC_FULL(acc));
+                        if (kc == hi - 1) mma_commit(ACC_FULL(acc));
                     }
                     if (++s == STAGES) { s = 0; ph ^= 1; }
                 }
                 ++n_done;
-                u += k1 - k0;
             }
         }
         if (!ok && !dead && lane == 0) atomicCAS(&g_few_error, 0, ERR_MMA);
@@ -273,102 +408,102 @@ layer_kernel(const TcProblem p, const __grid_constant__ CUtensorMap tmX, const _
         // ================================ epilogue ================================
         const int L = (warp & 3) * 32 + lane;          // TMEM lane = weight column of the tile
         const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
-        const int n_tok = p.n_tok;
-        const size_t piece_floats = (size_t)2 * n_tok * 128;
+        const size_t ld1 = (size_t)p.ft * 128, slab1 = (size_t)p.rows * 2 * ld1, slab2 = (size_t)p.rows * p.d;
         bool ok = !dead;
-        int n_done = 0;
-        // gate weight of every token for active expert a; negative: the token did not choose it
-        auto set_gate = [&](unsigned a) {
-            named_bar_sync(1, 128);                    // the table's previous readers are done
-            if (L < n_tok) {
-                float g = a >= routed ? 1.f : -1.f;
-                if (a < routed) {
-                    const int e = sh.list[a];
-                    for (int j = 0; j < p.k; ++j)
-                        if (__ldcg(p.idx + (size_t)L * p.k + j) == e) g = __ldcg(p.w + (size_t)L * p.k + j);
-                }
-                sh.gate[L] = g;
-            }
-            named_bar_sync(1, 128);
-        };
-        auto put_h = [&](unsigned a, int col, int t, float v1, float v3) {
-            const float g = sh.gate[t];
-            if (col < p.f) p.h[((size_t)a * n_tok + t) * p.f + col] = __float2bfloat16_rn(g < 0.f ? 0.f : g * silu(v1) * v3);
-        };
-        auto put_out = [&](int col, int t, float v) {
-            if (col < p.d) p.out[(size_t)t * p.d + col] = __float2bfloat16_rn(v);
-        };
+        int n_done = 0, n_items = 0;
 #pragma unroll 1
         for (int stage = 1; stage <= 2; ++stage) {
-            const Runs &r = stage == 1 ? r1 : r2;
-            const unsigned lo = stage == 1 ? u1_lo : u2_lo, hi = stage == 1 ? u1_hi : u2_hi;
-            for (unsigned u = lo; u < hi;) {
-                const unsigned tile = u / r.per, k0 = u - tile * r.per, k1 = min(r.per, k0 + (hi - u));
-                const unsigned a = stage == 1 ? tile / p.ft : 0;
-                const int col = (int)(stage == 1 ? tile - a * p.ft : tile) * 128 + L;
-                const bool whole = k1 - k0 == r.per;
+            for (;;) {
+                // every thread takes the same way through the named barriers, time-out or not
+                ok = ok && mbar_wait(QUEUED(n_items % QUEUE), (n_items / QUEUE) & 1);
+                named_bar_sync(1, 128);
+                if (!ok) sh.last = -1;
+                named_bar_sync(1, 128);
+                if (sh.last == -1) { ok = false; break; }
+                const unsigned item = *reinterpret_cast<volatile uint32_t *>(&sh.queue[n_items % QUEUE]);
+                ++n_items;
+                if (item == NO_ITEM) break;
                 const int acc = n_done & 1;
-                if (stage == 1 && whole) set_gate(a);
-                if (ok) ok = mbar_wait(ACC_FULL(acc), (n_done >> 1) & 1);
-                ok = __all_sync(0xffffffffu, ok);
-                tc_fence_after_sync();
                 const uint32_t d0 = tmem + lane_base + acc * 2 * NP;
-                float *piece = p.pieces + (2 * (size_t)cta + (tile == lo / r.per ? 0 : 1)) * piece_floats + L;
-#pragma unroll 1
-                for (int c = 0; c < NP && c < n_tok; c += 16) {
-                    uint32_t v1[16], v3[16];
-                    if (ok) {
-                        tmem_ld16(d0 + c, v1);
-                        if (stage == 1) tmem_ld16(d0 + NP + c, v3);
+                const bool landed = __all_sync(0xffffffffu, mbar_wait(ACC_FULL(acc), (n_done >> 1) & 1));
+                ok = ok && landed;
+                tc_fence_after_sync();
+                ++n_done;
+                if (stage == 2) {
+                    const unsigned j = item % p.nt, q = item / p.nt, g = q / it2.split, ks = q - g * it2.split;
+                    unsigned a;
+                    int row0;
+                    const int n = group_of(g, a, row0), col = (int)j * 128 + L;
+                    float *y = p.pieces + ks * slab2 + (size_t)row0 * p.d + col;
+                    for (int c = 0; c < n && landed; c += 16) {
+                        uint32_t v[16];
+                        tmem_ld16(d0 + c, v);
                         tmem_wait_ld();
-                    }
-                    if (!ok) continue;
+                        if (col < p.d)
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        const int t = c + j;
-                        if (t >= n_tok) continue;
-                        const float x1 = __uint_as_float(v1[j]), x3 = __uint_as_float(v3[j]);
-                        if (!whole) {
-                            piece[(size_t)t * 128] = x1;
-                            if (stage == 1) piece[(size_t)(n_tok + t) * 128] = x3;
-                        } else if (stage == 1) put_h(a, col, t, x1, x3);
-                        else put_out(col, t, x1);
+                            for (int i = 0; i < 16; ++i)
+                                if (c + i < n) y[(size_t)(c + i) * p.d] = __uint_as_float(v[i]);
+                    }
+                    tc_fence_before_sync();
+                    mbar_arrive(ACC_EMPTY(acc));
+                    continue;
+                }
+                const unsigned i1 = item % p.ft, q = item / p.ft, a = q / it1.split, ks = q - a * it1.split;
+                int row0;
+                const int n = rows_of(a, row0), col = (int)i1 * 128 + L;
+                float *piece = p.pieces + (size_t)row0 * 2 * ld1 + col;          // of split 0
+                for (int r0 = 0; r0 < n && landed; r0 += 8) {
+                    uint32_t v1[8], v3[8];
+#pragma unroll
+                    for (int r = 0; r < 8; ++r) {
+                        const int rr = min(r0 + r, n - 1), t = a < routed ? sh.token[row0 + rr] : rr;
+                        tmem_ld1(d0 + t, v1[r]);
+                        tmem_ld1(d0 + NP + t, v3[r]);
+                    }
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int r = 0; r < 8; ++r) {
+                        if (r0 + r >= n) break;
+                        const float x1 = __uint_as_float(v1[r]), x3 = __uint_as_float(v3[r]);
+                        if (it1.split > 1) {
+                            float *o = piece + ks * slab1 + (size_t)(r0 + r) * 2 * ld1;
+                            o[0] = x1;
+                            o[ld1] = x3;
+                        } else if (col < p.f) p.h[(size_t)(row0 + r0 + r) * p.f + col] = __float2bfloat16_rn(silu(x1) * x3);
                     }
                 }
                 tc_fence_before_sync();
                 mbar_arrive(ACC_EMPTY(acc));
-                ++n_done;
-                u += k1 - k0;
-                if (whole) continue;
-                // a shared tile: whoever brings the last piece sums them all, in order
-                __threadfence();
-                named_bar_sync(1, 128);
-                const unsigned c_lo = r.owner(tile * r.per), c_hi = r.owner(tile * r.per + r.per - 1);
-                if (L == 0) sh.last = atomicAdd((stage == 1 ? p.tickets1 : p.tickets2) + tile, 1u) == c_hi - c_lo;
-                named_bar_sync(1, 128);
-                if (!sh.last) continue;
-                __threadfence();
-                if (stage == 1) set_gate(a);
-                if (!ok) continue;
-                // the first CTA's run reaches the tile after others unless it starts with it; the rest start inside it
-                const float *first = p.pieces + (2 * (size_t)c_lo + (r.start(c_lo) / r.per == tile ? 0 : 1)) * piece_floats + L;
-                for (int t = 0; t < n_tok; ++t) {
-                    float x1 = __ldcg(first + (size_t)t * 128), x3 = stage == 1 ? __ldcg(first + (size_t)(n_tok + t) * 128) : 0.f;
-#pragma unroll 4
-                    for (unsigned c = c_lo + 1; c <= c_hi; ++c) {
-                        const float *q = p.pieces + 2 * (size_t)c * piece_floats + L;
-                        x1 += __ldcg(q + (size_t)t * 128);
-                        if (stage == 1) x3 += __ldcg(q + (size_t)(n_tok + t) * 128);
-                    }
-                    if (stage == 1) put_h(a, col, t, x1, x3);
-                    else put_out(col, t, x1);
-                }
             }
-            if (stage == 1) {
-                fence_proxy_async_all();               // h is read by bulk copies
-                __threadfence();
+            // h is read by bulk copies, the pieces and y by ordinary loads
+            auto arrive = [&](int bar) {
+                if (stage == 1) fence_proxy_async_all();
                 named_bar_sync(1, 128);
-                if (L == 0 && !dead) atomicAdd(p.bars + 1, 1u);
+                if (L == 0 && !dead) {
+                    __threadfence();
+                    atomicAdd(p.bars + bar, 1u);
+                }
+            };
+            arrive(stage);
+            if (stage == 1 && it1.split > 1) {
+                // tiles cut along their reduction: all CTAs sum the pieces, in order, and write h
+                if (L == 0 && !dead && !grid_wait(p.bars + 1, gridDim.x)) atomicCAS(&g_few_error, 0, ERR_GRID);
+                named_bar_sync(1, 128);
+                const unsigned elems = dead ? 0u : (unsigned)p.rows * (unsigned)p.f;
+                for (unsigned u = blockIdx.x * 128 + L; u < elems; u += gridDim.x * 128) {
+                    const unsigned r = u / p.f, c = u - r * p.f;
+                    const float *o = p.pieces + (size_t)r * 2 * ld1 + c;
+                    float v1[16], v3[16], x1 = 0.f, x3 = 0.f;
+#pragma unroll
+                    for (unsigned z = 0; z < 16; ++z) {
+                        v1[z] = z < it1.split ? __ldcg(o + z * slab1) : 0.f;
+                        v3[z] = z < it1.split ? __ldcg(o + z * slab1 + ld1) : 0.f;
+                    }
+#pragma unroll
+                    for (unsigned z = 0; z < 16; ++z) { x1 += v1[z]; x3 += v3[z]; }
+                    p.h[u] = __float2bfloat16_rn(silu(x1) * x3);
+                }
+                arrive(3);
             }
         }
         if (!ok && !dead) atomicCAS(&g_few_error, 0, ERR_EPILOGUE);
@@ -376,6 +511,62 @@ layer_kernel(const TcProblem p, const __grid_constant__ CUtensorMap tmX, const _
     tc_fence_before_sync();
     __syncthreads();
     if (warp == 1) { tc_fence_after_sync(); tmem_dealloc(tmem, C::COLS); }
+    // ---- stage 3: the weighted sum ------------------------------------------------------------------------------------------------
+    if (tid == 0 && !dead && !grid_wait(p.bars + 2, gridDim.x)) atomicCAS(&g_few_error, 0, ERR_GRID);
+    __syncthreads();
+    if (dead) return;
+    const size_t slab = (size_t)p.rows * p.d;
+    const int n = p.k + p.shared;
+    const long long threads = (long long)gridDim.x * TC_THREADS, me = (long long)blockIdx.x * TC_THREADS + tid;
+    // V columns a thread, J choices' pieces (four each) in flight
+    auto weighted_sum = [&](auto v_, auto j_) {
+        constexpr int V = decltype(v_)::value, J = decltype(j_)::value;
+        const int per_row = p.d / V;
+        for (long long u = me; u < (long long)p.n_tok * per_row; u += threads) {
+            const int t = (int)(u / per_row), c = (int)(u - (long long)t * per_row) * V;
+            float sum[V] = {};
+            for (int j0 = 0; j0 < n; j0 += J) {
+                float y[J][V] = {}, g[J];
+                for (unsigned z0 = 0; z0 < it2.split; z0 += 4) {
+                    float v[J][4][V];
+#pragma unroll
+                    for (int j = 0; j < J; ++j) {
+                        const bool in = j0 + j < n, own = j0 + j >= p.k;
+                        const size_t row = !in ? 0 : own ? choices + t : sh.row[t * p.k + j0 + j];
+                        const float *src = p.pieces + row * p.d + c;
+                        if (z0 == 0) g[j] = !in || own ? 1.f : __ldcg(p.w + (size_t)t * p.k + j0 + j);
+#pragma unroll
+                        for (unsigned z = 0; z < 4; ++z) {
+                            const bool ld = in && z0 + z < it2.split;
+                            if constexpr (V == 4) {
+                                const float4 q = ld ? __ldcg(reinterpret_cast<const float4 *>(src + (z0 + z) * slab)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                                v[j][z][0] = q.x; v[j][z][1] = q.y; v[j][z][2] = q.z; v[j][z][3] = q.w;
+                            } else v[j][z][0] = ld ? __ldcg(src + (z0 + z) * slab) : 0.f;
+                        }
+                    }
+#pragma unroll
+                    for (int j = 0; j < J; ++j)
+#pragma unroll
+                        for (int z = 0; z < 4; ++z)
+#pragma unroll
+                            for (int i = 0; i < V; ++i) y[j][i] += v[j][z][i];
+                }
+#pragma unroll
+                for (int j = 0; j < J; ++j)
+                    if (j0 + j < n)
+#pragma unroll
+                        for (int i = 0; i < V; ++i) sum[i] = fmaf(g[j], y[j][i], sum[i]);
+            }
+            __nv_bfloat16 *o = p.out + (size_t)t * p.d + c;
+            if constexpr (V == 4) {
+                const __nv_bfloat162 lo = __floats2bfloat162_rn(sum[0], sum[1]), hi = __floats2bfloat162_rn(sum[2], sum[3]);
+                *reinterpret_cast<uint2 *>(o) = make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
+            } else *o = __float2bfloat16_rn(sum[0]);
+        }
+    };
+    // one column a thread while that is at most one round (latency), four beyond
+    if ((long long)p.n_tok * p.d <= threads) weighted_sum(std::integral_constant<int, 1>{}, std::integral_constant<int, 9>{});
+    else weighted_sum(std::integral_constant<int, 4>{}, std::integral_constant<int, 4>{});
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------------
@@ -390,39 +581,42 @@ static int sm_count() {
 
 struct TcLayout {
     size_t part, idx, w, counters, h, pieces, total;
-    int n_counters, active_max, grid;
+    int rows, split_cap, grid;
 };
 static TcLayout tc_layout(int n_tok, int d, int f, int E, int k, int shared) {
     TcLayout L{};
+    const int ft = (f + 127) / 128;
     L.grid = sm_count();
-    L.active_max = (n_tok * k < E ? n_tok * k : E) + shared;
-    L.n_counters = 2 + L.active_max * ((f + 127) / 128) + (d + 127) / 128;
+    L.rows = n_tok * (k + shared);
+    // pieces cost 8 bytes per row and weight column and item; many rows come with many tiles, which need no cutting
+    L.split_cap = 4608 / L.rows < 1 ? 1 : (4608 / L.rows > 16 ? 16 : 4608 / L.rows);
+    const size_t wide = (size_t)2 * ft * 128 > (size_t)d ? (size_t)2 * ft * 128 : (size_t)d;
     size_t o = 0;
     L.part = o;     o += up256((size_t)gate_slices(n_tok, d, E) * n_tok * E * sizeof(double));
     L.idx = o;      o += up256((size_t)n_tok * k * 4);
     L.w = o;        o += up256((size_t)n_tok * k * 4);
-    L.counters = o; o += up256((size_t)L.n_counters * 4);
-    L.h = o;        o += up256((size_t)L.active_max * n_tok * f * 2);
-    L.pieces = o;   o += up256((size_t)2 * L.grid * 2 * n_tok * 128 * 4);
+    L.counters = o; o += up256(N_COUNTERS * 4);
+    L.h = o;        o += up256((size_t)L.rows * f * 2);
+    L.pieces = o;   o += up256((size_t)L.split_cap * L.rows * wide * 4);       // stage 1's are dead when stage 2's y are written
     L.total = o;
     return L;
 }
 
 static bool tc_supported(int d, int f, int E, int dtype) {
     return dtype == FDMLA_BF16 && d % 64 == 0 && f % 64 == 0 && (long long)E * d < (1LL << 31) && (long long)E * f < (1LL << 31) &&
-           (long long)(E + 1) * ((f + 127) / 128) * (d / 64) < (1LL << 31) && (long long)(E + 1) * ((d + 127) / 128) * ((f + 127) / 128) < (1LL << 31);
+           f <= 65535 * 128 && (long long)(E + 1) * ((f + 127) / 128) * 16 < (1LL << 31) && (long long)(E + 66) * ((d + 127) / 128) * 16 < (1LL << 31);
 }
 static bool tc_aligned(const Args &a) {
     return ((reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.W1) | reinterpret_cast<uintptr_t>(a.W3) |
              reinterpret_cast<uintptr_t>(a.W2) | reinterpret_cast<uintptr_t>(a.S1) | reinterpret_cast<uintptr_t>(a.S3) |
-             reinterpret_cast<uintptr_t>(a.S2)) & 15) == 0;
+             reinterpret_cast<uintptr_t>(a.S2)) & 15) == 0 && (reinterpret_cast<uintptr_t>(a.out) & 7) == 0;
 }
 
 template <int NP>
-static int launch_layer(const TcProblem &p, const Args &a, int grid, int active_max, cudaStream_t s) {
+static int launch_layer(const TcProblem &p, const Args &a, int grid, cudaStream_t s) {
     CUtensorMap tmX, tmH, tm[6];
     if (!make_tensor_map_bf16(&tmX, a.x, a.n_tok, a.d, NP) ||
-        !make_tensor_map_bf16(&tmH, p.h, (long long)active_max * a.n_tok, a.f, NP)) return FDMLA_ERR_CUDA;
+        !make_tensor_map_bf16(&tmH, p.h, p.rows, a.f, 16)) return FDMLA_ERR_CUDA;
     const void *base[6] = {a.W1, a.W3, a.W2, a.S1, a.S3, a.S2};
     for (int i = 0; i < 6; ++i) {
         if (i >= 3 && !a.shared) { tm[i] = tm[i - 3]; continue; }
@@ -461,17 +655,16 @@ static int run_tensor(const Args &a, uint8_t *ws, cudaStream_t s) {
     p.part = part;
     p.idx = reinterpret_cast<int32_t *>(ws + L.idx);
     p.w = reinterpret_cast<float *>(ws + L.w);
-    p.bars = counters; p.tickets1 = counters + 2; p.tickets2 = p.tickets1 + (size_t)L.active_max * p.ft;
+    p.bars = counters; p.next = counters + 4;
+    p.rows = L.rows; p.split_cap = L.split_cap;
     p.h = reinterpret_cast<__nv_bfloat16 *>(ws + L.h);
     p.pieces = reinterpret_cast<float *>(ws + L.pieces);
     p.out = static_cast<__nv_bfloat16 *>(a.out);
-    gate_kernel<__nv_bfloat16><<<dim3((a.E + 31) / 32, p.slices, (a.n_tok + GATE_TOK - 1) / GATE_TOK), GATE_THREADS, 0, s>>>(
-        static_cast<const __nv_bfloat16 *>(a.x), a.Wg, part, counters, L.n_counters, a.n_tok, a.d, a.E);
-    if (check_launch() != FDMLA_OK) return FDMLA_ERR_CUDA;
-    if (a.n_tok <= 16) return launch_layer<16>(p, a, L.grid, L.active_max, s);
-    if (a.n_tok <= 32) return launch_layer<32>(p, a, L.grid, L.active_max, s);
-    if (a.n_tok <= 64) return launch_layer<64>(p, a, L.grid, L.active_max, s);
-    return launch_layer<128>(p, a, L.grid, L.active_max, s);
+    if (launch_gate<__nv_bfloat16>(a.x, a.Wg, part, counters, N_COUNTERS, a.n_tok, a.d, a.E, p.slices, s) != FDMLA_OK) return FDMLA_ERR_CUDA;
+    if (a.n_tok <= 16) return launch_layer<16>(p, a, L.grid, s);
+    if (a.n_tok <= 32) return launch_layer<32>(p, a, L.grid, s);
+    if (a.n_tok <= 64) return launch_layer<64>(p, a, L.grid, s);
+    return launch_layer<128>(p, a, L.grid, s);
 }
 
 }  // namespace few

@@ -105,6 +105,8 @@ CASES = [
     (65, 320, 64, 33, 32, False, torch.bfloat16),
     (128, 256, 192, 300, 8, True, torch.bfloat16),
     (128, 64, 64, 3, 1, True, torch.bfloat16),
+    (4, 4096, 256, 8, 2, True, torch.bfloat16),               # few tiles, long sums: many pieces per tile
+    (128, 1024, 512, 4, 2, True, torch.bfloat16),             # more than 64 tokens per expert
     (3, 100, 36, 7, 2, True, torch.bfloat16),                 # widths the tensor cores do not take
     (1, 33, 5, 2, 1, False, torch.bfloat16),
     (1, 64, 128, 8, 2, True, torch.float32),
