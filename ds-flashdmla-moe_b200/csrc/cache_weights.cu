@@ -324,14 +324,22 @@ __global__ void __launch_bounds__(256) move_kernel(uint8_t *__restrict__ pool, f
 
 }  // namespace cw
 
+}  // namespace fdmla
+
+#include "cache_weights_tc.cuh"
+
+namespace fdmla {
+
 int cache_error_flag(int reset) {
-    int v = 0;
-    if (cudaMemcpyFromSymbol(&v, cw::g_cache_error, sizeof(int)) != cudaSuccess) return -1;
-    if (reset && v != 0) {
+    int page = 0, wait = 0;
+    if (cudaMemcpyFromSymbol(&page, cw::g_cache_error, sizeof(int)) != cudaSuccess ||
+        cudaMemcpyFromSymbol(&wait, cw::g_acc_error, sizeof(int)) != cudaSuccess) return -1;
+    if (reset && (page | wait)) {
         const int zero = 0;
-        if (cudaMemcpyToSymbol(cw::g_cache_error, &zero, sizeof(int)) != cudaSuccess) return -1;
+        if (cudaMemcpyToSymbol(cw::g_cache_error, &zero, sizeof(int)) != cudaSuccess ||
+            cudaMemcpyToSymbol(cw::g_acc_error, &zero, sizeof(int)) != cudaSuccess) return -1;
     }
-    return v;
+    return wait ? wait : page;
 }
 
 }  // namespace fdmla
@@ -343,8 +351,11 @@ static bool pages_ok(int B, int page_size, int max_pages, int num_pages) {
 }
 
 extern "C" size_t fdmla_cache_accumulate_workspace_bytes(int B, int H, int Sq, int d_qk, int page_size, int max_pages, int dtype) {
-    (void)B; (void)H; (void)Sq; (void)d_qk; (void)page_size; (void)max_pages; (void)dtype;
-    return 0;
+    if (B <= 0 || H <= 0 || Sq <= 0 || d_qk <= 0 || page_size <= 0 || max_pages <= 0) return 0;
+    if (!cw::accumulate_tc_supported(B, (long long)H * Sq, d_qk, page_size, 1, dtype)) return 0;
+    const long long cap = (long long)page_size * max_pages;
+    const int splits = cw::row_splits(B, (long long)H * Sq, cap);
+    return splits > 1 ? (size_t)splits * B * cap * sizeof(float) : 0;
 }
 
 extern "C" int fdmla_cache_accumulate(const void *Q, const void *kv_pool, const int32_t *page_table, const int32_t *seqlens,
@@ -357,14 +368,20 @@ extern "C" int fdmla_cache_accumulate(const void *Q, const void *kv_pool, const 
     if (!Q || !kv_pool || !page_table || !seqlens || !m || !l || !weights) return FDMLA_ERR_INVALID;
     if (!pages_ok(B, page_size, max_pages, num_pages) || (long long)H * Sq > 2147483647LL) return FDMLA_ERR_UNSUPPORTED;
     if (workspace_bytes < fdmla_cache_accumulate_workspace_bytes(B, H, Sq, d_qk, page_size, max_pages, dtype)) return FDMLA_ERR_WORKSPACE;
-    (void)workspace;
+    if (workspace_bytes > 0 && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255))) return FDMLA_ERR_WORKSPACE;
     cw::AccProblem p{};
     p.Q = Q; p.pool = kv_pool; p.m = m; p.l = l; p.weights = weights;
     p.pg = cw::Pages{page_table, seqlens, page_size, max_pages, num_pages};
     p.B = B; p.R = H * Sq; p.Sq = Sq; p.d = d_qk; p.causal = causal ? 1 : 0;
     p.scale_log2 = scale * 1.4426950408889634f;
     cudaStream_t s = (cudaStream_t)stream;
-    if (fdmla_get_backend() == FDMLA_BACKEND_TENSOR) return FDMLA_ERR_UNSUPPORTED;
+    const bool tc = cw::accumulate_tc_supported(B, p.R, d_qk, page_size, num_pages, dtype) &&
+                    ((reinterpret_cast<uintptr_t>(Q) | reinterpret_cast<uintptr_t>(kv_pool)) & 15) == 0;
+    if (fdmla_get_backend() == FDMLA_BACKEND_TENSOR && !tc) return FDMLA_ERR_UNSUPPORTED;
+    if (tc && tensor_kernels_allowed()) {
+        note_kernel("tcgen05");
+        return cw::run_accumulate_tc(p, workspace, s);
+    }
     note_kernel("portable");
     const long long smem = 32LL * (d_qk + 1) * 4;
     if (smem > kMaxSmemPerBlock) return FDMLA_ERR_UNSUPPORTED;

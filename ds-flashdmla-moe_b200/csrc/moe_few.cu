@@ -28,16 +28,18 @@ constexpr int MAX_T = 128;
 __device__ __forceinline__ float silu(float x) { return x / (1.f + __expf(-x)); }
 
 // ---- gate: logits in 64 bits -------------------------------------------------------------------------------------------
-// Block (32 experts, one of gridDim.y slices of d, 8 tokens): a lane owns an expert, a warp every 16th row of the slice.
-// part[s, t, e] holds slice s's share of the logit.  The widths of real gates leave a few hundred rows per block, so that
-// every warp has most of its loads in flight at once.  All blocks together also clear the counters of the kernel behind.
-constexpr int GATE_THREADS = 512, GATE_TOK = 8, GATE_ROWS = 256, MAX_SLICES = 32;
+// Block (32 experts, one of gridDim.y slices of d, TOK tokens): a lane owns an expert, a warp every 16th of ROWS rows at a time,
+// whose loads are all in flight at once.  part[s, t, e] holds slice s's share of the logit.  All blocks together also clear the
+// counters of the kernel behind.  For one token 512 rows and one block per SM (64 registers, as two blocks would leave, spill and
+// cost 3 us of 23 .. 150); for more 256 rows, 8 tokens and two blocks.
+constexpr int GATE_THREADS = 512, GATE_TOK = 8, MAX_SLICES = 32;
 
-template <typename T, int TOK>
-__global__ void __launch_bounds__(GATE_THREADS) gate_kernel(const T *__restrict__ x, const float *__restrict__ Wg,
+template <typename T, int TOK, int ROWS>
+__global__ void __launch_bounds__(GATE_THREADS, TOK == 1 ? 1 : 2) gate_kernel(const T *__restrict__ x, const float *__restrict__ Wg,
                                                             double *__restrict__ part, unsigned *__restrict__ counters,
                                                             int n_counters, int n_tok, int d, int E) {
-    __shared__ double s_x[GATE_ROWS][TOK];                       // later the warps' partial sums
+    __shared__ double s_x[ROWS][TOK];                       // later the warps' partial sums
+    ptx::launch_dependents();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int e = blockIdx.x * 32 + lane, t0 = blockIdx.z * TOK;
     {
@@ -49,22 +51,22 @@ __global__ void __launch_bounds__(GATE_THREADS) gate_kernel(const T *__restrict_
     double acc[TOK];
 #pragma unroll
     for (int j = 0; j < TOK; ++j) acc[j] = 0.0;
-    for (int r0 = lo; r0 < hi; r0 += GATE_ROWS) {
-        const int rows = hi - r0 < GATE_ROWS ? hi - r0 : GATE_ROWS;
-        float wv[GATE_ROWS / 16];
+    for (int r0 = lo; r0 < hi; r0 += ROWS) {
+        const int rows = hi - r0 < ROWS ? hi - r0 : ROWS;
+        float wv[ROWS / 16];
 #pragma unroll
-        for (int i = 0; i < GATE_ROWS / 16; ++i) {
+        for (int i = 0; i < ROWS / 16; ++i) {
             const int r = warp + 16 * i;
             wv[i] = (r < rows && e < E) ? __ldg(Wg + (size_t)(r0 + r) * E + e) : 0.f;
         }
         __syncthreads();
-        for (int i = threadIdx.x; i < GATE_ROWS * TOK; i += GATE_THREADS) {
-            const int r = i % GATE_ROWS, j = i / GATE_ROWS;
+        for (int i = threadIdx.x; i < ROWS * TOK; i += GATE_THREADS) {
+            const int r = i % ROWS, j = i / ROWS;
             s_x[r][j] = (r < rows && t0 + j < n_tok) ? (double)to_f32(x[(size_t)(t0 + j) * d + r0 + r]) : 0.0;
         }
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < GATE_ROWS / 16; ++i) {
+        for (int i = 0; i < ROWS / 16; ++i) {
             const int r = warp + 16 * i;
             if (r >= rows) break;
             const double wd = (double)wv[i];
@@ -97,15 +99,15 @@ template <typename T>
 static int launch_gate(const void *x, const float *Wg, double *part, unsigned *counters, int n_counters, int n_tok, int d, int E,
                        int slices, cudaStream_t s) {
     const dim3 grid((E + 31) / 32, slices, (n_tok + GATE_TOK - 1) / GATE_TOK);
-    if (n_tok == 1) gate_kernel<T, 1><<<grid, GATE_THREADS, 0, s>>>(static_cast<const T *>(x), Wg, part, counters, n_counters, n_tok, d, E);
-    else gate_kernel<T, GATE_TOK><<<grid, GATE_THREADS, 0, s>>>(static_cast<const T *>(x), Wg, part, counters, n_counters, n_tok, d, E);
+    if (n_tok == 1) gate_kernel<T, 1, 512><<<grid, GATE_THREADS, 0, s>>>(static_cast<const T *>(x), Wg, part, counters, n_counters, n_tok, d, E);
+    else gate_kernel<T, GATE_TOK, 256><<<grid, GATE_THREADS, 0, s>>>(static_cast<const T *>(x), Wg, part, counters, n_counters, n_tok, d, E);
     return check_launch();
 }
 
-// slices of d: enough blocks for every SM, at least 64 rows each
+// slices of d: one round of blocks, at least 64 rows each
 static int gate_slices(int n_tok, int d, int E) {
     const int blocks = ((E + 31) / 32) * ((n_tok + GATE_TOK - 1) / GATE_TOK);
-    int s = (2 * kNumSMs + blocks - 1) / blocks;
+    int s = n_tok == 1 ? kNumSMs / blocks : (2 * kNumSMs + blocks - 1) / blocks;
     if (s > MAX_SLICES) s = MAX_SLICES;
     if (s > d / 64) s = d / 64;
     return s < 1 ? 1 : s;
@@ -151,14 +153,23 @@ __device__ __forceinline__ void topk_warp(unsigned long long *key, int E, int k,
     if (lane < k) { idx[lane] = my_i; w[lane] = my_w / sum; }
 }
 
-// Sum of a logit's slices, in order, all loads in flight.
-__device__ __forceinline__ double logit(const double *__restrict__ part, int slices, size_t stride) {
-    double v[MAX_SLICES], z = 0.0;
+// Sort keys of one token's logits into key [E]: sums of the slices, in order, eight loads in flight (all 32 at once take 1 us
+// longer for the few slices of a narrow layer and gain nothing for wide ones).  Returns whether this thread saw a NaN.
+__device__ __forceinline__ bool token_keys(const double *__restrict__ part, int slices, size_t stride, int E, unsigned long long *key) {
+    bool nan = false;
+    for (int e = threadIdx.x; e < E; e += blockDim.x) {
+        double z = 0.0;
+        for (int s0 = 0; s0 < slices; s0 += 8) {
+            double v[8];
 #pragma unroll
-    for (int s = 0; s < MAX_SLICES; ++s) v[s] = s < slices ? part[(size_t)s * stride] : 0.0;
+            for (int s = 0; s < 8; ++s) v[s] = s0 + s < slices ? part[(size_t)(s0 + s) * stride + e] : 0.0;
 #pragma unroll
-    for (int s = 0; s < MAX_SLICES; ++s) z += v[s];
-    return z;
+            for (int s = 0; s < 8; ++s) z += v[s];
+        }
+        key[e] = logit_key(z);
+        nan |= isnan(z);
+    }
+    return nan;
 }
 
 // ---- the layer on CUDA cores: any type, any width ------------------------------------------------------------------------
@@ -166,13 +177,7 @@ __global__ void __launch_bounds__(128) route_kernel(const double *__restrict__ p
                                                     float *__restrict__ w, int n_tok, int E, int k) {
     extern __shared__ unsigned long long s_key[];
     const int t = blockIdx.x;
-    bool nan = false;
-    for (int e = threadIdx.x; e < E; e += blockDim.x) {
-        const double z = logit(part + (size_t)t * E + e, slices, (size_t)n_tok * E);
-        s_key[e] = logit_key(z);
-        nan |= isnan(z);
-    }
-    nan = __syncthreads_or(nan);
+    const bool nan = __syncthreads_or(token_keys(part + (size_t)t * E, slices, (size_t)n_tok * E, E, s_key));
     if (threadIdx.x < 32) topk_warp(s_key, E, k, nan, idx + (size_t)t * k, w + (size_t)t * k, threadIdx.x);
 }
 

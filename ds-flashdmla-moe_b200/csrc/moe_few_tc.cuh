@@ -34,34 +34,34 @@ constexpr int MAX_E = 2048;
 enum { ERR_PRODUCER = 41, ERR_MMA = 42, ERR_EPILOGUE = 43, ERR_GRID = 44 };
 __device__ int g_few_error = 0;
 
-// NP: tokens of the call rounded up to the width of the MMA's N side in stage 1.  The ring takes 180 to 200 KB of shared memory;
+// NP: tokens of the call rounded up to the width of the MMA's N side in stage 1.  The ring takes 192 to 216 KB of shared memory;
 // about 50 KB in flight per SM cover the latency of HBM at full bandwidth.
 constexpr int GROUP = 64;                             // rows of h in one accumulator of stage 2
+constexpr int QUEUE = 16;                             // items under way: at most 6 ring stages + 2 accumulators + 2
+constexpr unsigned NO_ITEM = 0xffffffffu;
+constexpr int N_COUNTERS = 6;
+
+template <int NP> struct TcShared {                   // behind the ring
+    static constexpr int ROWS = NP * 32, EXPERTS = ROWS < MAX_E ? ROWS : MAX_E;      // k <= 32
+    uint64_t bars[2 * 6 + 4 + QUEUE];
+    uint32_t tmem, queue[QUEUE], ahead[6], scan[16];
+    int n_routed, n_groups, last, dead;
+    uint16_t expert[EXPERTS];                         // routed experts, ascending
+    uint16_t first[EXPERTS + 1];                      // their first rows of h
+    uint16_t group[EXPERTS + 2 + ROWS / GROUP];       // routed expert (or n_routed: the shared one) | second group << 15
+    uint16_t row[ROWS];                               // of every choice (t, j)
+    uint8_t token[ROWS];                              // of every row of h
+};
 template <int NP> struct Cfg {
     static constexpr int GN = NP < GROUP ? NP : GROUP;
     static constexpr int B_BYTES = (NP > 2 * GN ? NP : 2 * GN) * 128;   // 64 activations of all tokens / 2 x 64 of a group
     static constexpr int STAGE = A_BYTES + B_BYTES;
-    static constexpr int STAGES = NP <= 32 ? 5 : 4;
+    static constexpr int STAGES = NP == 16 ? 6 : (NP == 32 ? 5 : 4);
     static constexpr int COLS = 4 * NP;               // tensor memory: two buffers of (D1, D3)
-    static constexpr int SMEM = 1024 + STAGES * STAGE + 25600;
+    static constexpr int SMEM = 1024 + STAGES * STAGE + (int)sizeof(TcShared<NP>);
     static_assert(SMEM <= kMaxSmemPerBlock, "shared memory overflow");
+    static_assert(STAGES * STAGE >= 16384 + MAX_E * 18 + 2 * TcShared<NP>::ROWS, "the tables behind the top-k overflow the ring");
 };
-constexpr int MAX_ROWS = MAX_T * 32, MAX_GROUPS = MAX_E + 2 + MAX_ROWS / GROUP;
-constexpr int QUEUE = 16;                             // items under way: at most 5 ring stages + 2 accumulators + 2
-constexpr unsigned NO_ITEM = 0xffffffffu;
-constexpr int N_COUNTERS = 6;
-
-struct TcShared {                                     // behind the ring
-    uint64_t bars[2 * 5 + 4 + QUEUE];
-    uint32_t tmem, queue[QUEUE], ahead[5], scan[16];
-    int n_routed, n_groups, last, dead;
-    uint16_t expert[MAX_E];                           // routed experts, ascending
-    uint16_t first[MAX_E + 1];                        // their first rows of h
-    uint16_t group[MAX_GROUPS];                       // routed expert (or n_routed: the shared one) | second group << 15
-    uint8_t token[MAX_ROWS];                          // of every row of h
-    uint16_t row[MAX_ROWS];                           // of every choice (t, j)
-};
-static_assert(sizeof(TcShared) <= 25600, "TcShared outgrew its space");
 
 struct TcProblem {
     int n_tok, d, f, E, k, shared, slices;
@@ -105,7 +105,7 @@ layer_kernel(const TcProblem p, const __grid_constant__ CUtensorMap tmX, const _
     constexpr int STAGES = C::STAGES, STAGE = C::STAGE;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *ring = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    TcShared &sh = *reinterpret_cast<TcShared *>(ring + STAGES * STAGE);
+    TcShared<NP> &sh = *reinterpret_cast<TcShared<NP> *>(ring + STAGES * STAGE);
     const uint32_t bar0 = smem_u32(sh.bars);
     auto FULL = [&](int s) { return bar0 + 8u * s; };
     auto EMPTY = [&](int s) { return bar0 + 8u * (STAGES + s); };
@@ -124,27 +124,21 @@ layer_kernel(const TcProblem p, const __grid_constant__ CUtensorMap tmX, const _
         fence_mbar_init();
     }
     if (warp == 1) { tmem_alloc(smem_u32(&sh.tmem), C::COLS); tmem_relinquish(); }
+    wait_for_primary();                                // the gate kernel's logits and zeroed counters
 
     // ---- top-k: one token per CTA, in shared memory that the ring uses later ---------------------------------------------------
     unsigned long long *s_key = reinterpret_cast<unsigned long long *>(ring);
     for (int t = blockIdx.x; t < p.n_tok; t += gridDim.x) {
-        bool nan = false;
-        for (int e = tid; e < p.E; e += TC_THREADS) {
-            const double z = logit(p.part + (size_t)t * p.E + e, p.slices, (size_t)p.n_tok * p.E);
-            s_key[e] = logit_key(z);
-            nan |= isnan(z);
-        }
-        nan = __syncthreads_or(nan);
+        const bool nan = __syncthreads_or(token_keys(p.part + (size_t)t * p.E, p.slices, (size_t)p.n_tok * p.E, p.E, s_key));
         if (warp == 0) topk_warp(s_key, p.E, p.k, nan, p.idx + (size_t)t * p.k, p.w + (size_t)t * p.k, lane);
         __syncthreads();
     }
     // which tokens chose an expert: a 128-bit mask each
     uint32_t(*s_mask)[4] = reinterpret_cast<uint32_t(*)[4]>(ring + 16384);
-    uint16_t *s_first = reinterpret_cast<uint16_t *>(ring + 16384 + MAX_E * 16);
+    uint16_t *s_first = reinterpret_cast<uint16_t *>(ring + 16384 + MAX_E * 16), *s_idx = s_first + MAX_E;
     for (int i = tid; i < p.E * 4; i += TC_THREADS) (&s_mask[0][0])[i] = 0u;
     if (tid == 0 && !sh.dead) {
-        __threadfence();
-        atomicAdd(p.bars, 1u);
+        red_release_gpu(p.bars);
         if (!grid_wait(p.bars, gridDim.x)) { sh.dead = 1; atomicCAS(&g_few_error, 0, ERR_GRID); }
     }
     tc_fence_before_sync();
@@ -156,6 +150,7 @@ layer_kernel(const TcProblem p, const __grid_constant__ CUtensorMap tmX, const _
     if (!dead)
         for (int i = tid; i < choices; i += TC_THREADS) {
             const int e = __ldcg(p.idx + i), t = i / p.k;
+            s_idx[i] = (uint16_t)e;
             atomicOr(&s_mask[e][t >> 5], 1u << (t & 31));
         }
     __syncthreads();
@@ -203,7 +198,7 @@ layer_kernel(const TcProblem p, const __grid_constant__ CUtensorMap tmX, const _
     __syncthreads();
     if (!dead)
         for (int i = tid; i < choices; i += TC_THREADS) {
-            const int e = __ldcg(p.idx + i), t = i / p.k;
+            const int e = s_idx[i], t = i / p.k;
             int r = s_first[e];
             for (int q = 0; q < t >> 5; ++q) r += __popc(s_mask[e][q]);
             r += __popc(s_mask[e][t >> 5] & ((1u << (t & 31)) - 1u));
@@ -295,8 +290,10 @@ layer_kernel(const TcProblem p, const __grid_constant__ CUtensorMap tmX, const _
                 }
             open = true;
         };
-        // the first items go by CTA number, so that each CTA knows which weights to have brought into L2: about 12 units
-        const unsigned fixed = min(max(it2.total / (4 * gridDim.x), 1u), (12 + it2.per / it2.split - 1) / max(it2.per / it2.split, 1u));
+        // the first items go by CTA number, so that each CTA knows which weights to have brought into L2: about 6 units beyond
+        // the ring's (29 MB in all; 16 were 1 to 2 us slower), a quarter of the work at most
+        const unsigned units = max(it2.per / it2.split, 1u);
+        const unsigned fixed = max(min(it2.total / (4 * gridDim.x), (STAGES + 6 + units - 1) / units), 1u);
         unsigned round = 0;
         auto prefetch = [&](unsigned item, unsigned skip) {
             const unsigned j = item % p.nt, q = item / p.nt, g = q / it2.split, ks = q - g * it2.split;
@@ -479,10 +476,7 @@ layer_kernel(const TcProblem p, const __grid_constant__ CUtensorMap tmX, const _
             auto arrive = [&](int bar) {
                 if (stage == 1) fence_proxy_async_all();
                 named_bar_sync(1, 128);
-                if (L == 0 && !dead) {
-                    __threadfence();
-                    atomicAdd(p.bars + bar, 1u);
-                }
+                if (L == 0 && !dead) red_release_gpu(p.bars + bar);
             };
             arrive(stage);
             if (stage == 1 && it1.split > 1) {
@@ -632,11 +626,13 @@ static int launch_layer(const TcProblem &p, const Args &a, int grid, cudaStream_
     cfg.blockDim = dim3(TC_THREADS);
     cfg.dynamicSmemBytes = Cfg<NP>::SMEM;
     cfg.stream = s;
-    cudaLaunchAttribute at;
-    at.id = cudaLaunchAttributeCooperative;
-    at.val.cooperative = 1;
-    cfg.attrs = &at;
-    cfg.numAttrs = 1;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeCooperative;
+    at[0].val.cooperative = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;     // set up while the gate kernel runs
+    at[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 2;
     if (cudaLaunchKernelEx(&cfg, layer_kernel<NP>, p, tmX, tmH, tm[0], tm[1], tm[2], tm[3], tm[4], tm[5]) != cudaSuccess) {
         cudaGetLastError();
         return FDMLA_ERR_CUDA;

@@ -156,6 +156,14 @@ __device__ __forceinline__ void bulk_wait_read() {
     asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(Pending) : "memory");
 }
 
+// Programmatic dependent launch: a kernel lets the next one on its stream start before it ends; that one waits here until the
+// first has ended and its writes are visible.  Without the launch attribute both do nothing.
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_primary() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// adds 1; everything the thread has done or has seen done (bar.sync) before is visible to whoever acquires the new value
+__device__ __forceinline__ void red_release_gpu(unsigned *p) {
+    asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(p) : "memory");
+}
 __device__ __forceinline__ uint32_t ld_acquire_gpu(const unsigned *p) {
     uint32_t v;
     asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
