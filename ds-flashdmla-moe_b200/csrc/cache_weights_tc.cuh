@@ -1,18 +1,18 @@
 // Attention weight per cached row on the tensor cores (included by cache_weights.cu): bf16, d a multiple of 64 up to 576, pages
 // a multiple of 64 rows.
 //
-// D = K Q^T with the keys as the M side: a thread of the epilogue owns one key and sums exp2(s - m) / l over the columns of its
-// accumulator row in registers - no reduction between threads, no atomics between tiles.  Tiles are 256 keys x up to 128 query
+// D = K Q^T with the keys as the M side: a thread of the epilogue owns one key and sums 2^(s - m) / l over the columns of its
+// accumulator row in registers - no reduction between threads, no atomics between tiles.  Tiles are 256 keys x up to 256 query
 // rows, computed by a pair of CTAs (cta_group::2): each CTA holds the accumulator rows of its own 128 keys, brings those keys
-// and HALF of the query rows, so that 128 queries x 576 take 74 KB instead of 147 and the ring beside them is deep enough to
+// and HALF of the query rows, so that 128 query rows x 576 take 74 KB instead of 147 and the ring beside them is deep enough to
 // cover the latency of HBM (four slots of one CTA alone would hold 64 KB in flight).
-//   ROWS = false  at most 128 query rows per sequence (a decode step): they stay in shared memory while the keys of the
+//   ROWS = false  at most 256 query rows per sequence (a decode step): they stay in shared memory while the keys of the
 //                 sequence stream past; a pair takes a contiguous run of tiles, at a change of sequence the queries are
 //                 exchanged chunk by chunk as the last MMAs release them.  Bound by reading the rows once.
-//   ROWS = true   more query rows (a prompt, a window of queries, more than 128 heads): a tile's keys stay and the query rows
-//                 stream, 128 at a time, the sums staying in registers; tiles are dealt out round robin and, when there are
+//   ROWS = true   more query rows (a prompt, a window of queries): a tile's keys stay and the query rows stream, 256 at a time (an
+//                 MMA costs about 60 cycles to issue: with 128 the issue, not the MMA, bounds), the sums staying in registers; tiles are dealt out round robin and, when there are
 //                 few, cut along the query rows into `splits` whose partial sums a second kernel adds in order.  Bound by the
-//                 MMAs, 2 * 256 * 128 * d operations per step.
+//                 MMAs, 2 * 256 * 256 * d operations per step.
 // Either way one operand is resident in chunks of 64 columns (RFULL / REMPTY per chunk) and the other one passes through the ring
 // (FULL / EMPTY per slot, in chunks of 64 columns too).
 //
@@ -27,7 +27,7 @@ bool make_tensor_map_bf16(CUtensorMap *m, const void *base, long long rows, int 
 
 namespace cw {
 
-constexpr int TC_THREADS = 192, KEYS = 256, QROWS = 128, MAX_CHUNKS = 9, MAX_SLOTS = 12;
+constexpr int TC_THREADS = 192, KEYS = 256, QROWS = 256, MAX_CHUNKS = 9, MAX_SLOTS = 12;
 constexpr int KEY_CHUNK = 128 * 128;                 // one CTA's 128 keys x 64 columns
 enum { ERR_PRODUCER = 51, ERR_MMA = 52, ERR_EPILOGUE = 53 };
 __device__ int g_acc_error = 0;
@@ -97,6 +97,13 @@ struct Walker {
         return (wraps ? p.a.Sq - 1 : q1) + n - p.a.Sq >= t0;
     }
 };
+
+// 2^x to two units in the last place, 0 for results below the normal numbers
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 
 template <bool ROWS>
 __global__ void __launch_bounds__(TC_THREADS, 1)
@@ -169,12 +176,20 @@ accumulate_kernel(const TcProblem p, const __grid_constant__ CUtensorMap tmQ, co
         const uint32_t full_lead = map_to_cta(FULL(0), 0), rfull_lead = map_to_cta(RFULL(0), 0);
         bool ok = !dead;
         int s = 0, use = 0, n_res = 0;
-        // row in the pool of the 64 keys lane & 3 of a tile (lanes 0..3 hold the four of them); a bad page reads page 0
-        auto locate = [&](int b, int t0, int n) {
-            const int t = t0 + 64 * (lane & 3);
-            if (t >= n) return 0;
-            const long long r = a.pg.row(b, t);
-            return r < 0 ? 0 : (int)r;
+        // page of the 64 keys number `lane & 3` of a tile; only looked at (row_of) a tile later, so that nobody waits for the load
+        auto page_of = [&](int b, int t0, int n) {
+            const int t = min(t0 + 64 * (lane & 3), n - 1);
+            return __ldg(a.pg.table + (size_t)b * a.pg.max_pages + t / a.pg.page_size);
+        };
+        // row in the pool of the tile's 64 keys number i; a bad page reads page 0
+        auto row_of = [&](int page, int t0, int n, int i) {
+            int pg = __shfl_sync(0xffffffffu, page, i);
+            const int t = t0 + 64 * i;
+            if (pg < 0 || pg >= a.pg.num_pages) {
+                if (t < n) g_cache_error = ERR_PAGE;
+                pg = 0;
+            }
+            return pg * a.pg.page_size + t % a.pg.page_size;
         };
         // this CTA's two blocks of 64 keys, columns 64 c .. + 63
         auto load_keys = [&](int r0, int r1, int halves, int c, uint32_t dst, uint32_t bar) {
@@ -184,9 +199,9 @@ accumulate_kernel(const TcProblem p, const __grid_constant__ CUtensorMap tmQ, co
         Walker<ROWS> w(p, sh, unit);
         while (ok && w.next(units)) {
             const int b = w.b;
-            int rows = locate(b, w.t0, w.n), r0 = 0, r1 = 0;
+            int page = page_of(b, w.t0, w.n), r0 = 0, r1 = 0;
             const int half_cols = p.n_cols / 2;
-            if (ROWS) { r0 = __shfl_sync(0xffffffffu, rows, 2 * rank); r1 = __shfl_sync(0xffffffffu, rows, 2 * rank + 1); }
+            if (ROWS) { r0 = row_of(page, w.t0, w.n, 2 * rank); r1 = row_of(page, w.t0, w.n, 2 * rank + 1); }
             const int halves0 = min(4, (w.n - w.t0 + 63) / 64);
             auto resident = [&](int c) {
                 if (n_res > 0) ok = ok && mbar_wait(REMPTY(c), (n_res - 1) & 1);
@@ -209,10 +224,10 @@ accumulate_kernel(const TcProblem p, const __grid_constant__ CUtensorMap tmQ, co
                     q_row = b * a.R + (w.r_lo + i) * QROWS + rank * half_cols;
                 } else {
                     const int t0 = w.t0 + i * KEYS;
-                    r0 = __shfl_sync(0xffffffffu, rows, 2 * rank);
-                    r1 = __shfl_sync(0xffffffffu, rows, 2 * rank + 1);
+                    r0 = row_of(page, t0, w.n, 2 * rank);
+                    r1 = row_of(page, t0, w.n, 2 * rank + 1);
                     halves = min(4, (w.n - t0 + 63) / 64);
-                    if (i + 1 < w.count) rows = locate(b, t0 + KEYS, w.n);       // the next tile's pages, ahead of time
+                    if (i + 1 < w.count) page = page_of(b, t0 + KEYS, w.n);      // the next tile's, ahead of time
                 }
                 for (int c = 0; c < p.chunks && ok; ++c) {
                     // the resident chunk is asked for one ring length behind the streaming ones: the last MMAs of the previous
@@ -290,17 +305,27 @@ accumulate_kernel(const TcProblem p, const __grid_constant__ CUtensorMap tmQ, co
         const uint32_t acc_empty_lead = map_to_cta(ACC_EMPTY(0), 0);
         bool ok = !dead;
         int n_done = 0;
-        // thread L fetches query row `row` of the tile that starts at r0: m log2(e), 1 / l and the last key it sees.  A row that
-        // sees nothing gets (inf, 0): every exponential is 0.
-        auto fetch = [&](int b, int n, int r0, float2 &ml, int &last) {
-            const int r = r0 + L;
-            ml = make_float2(CUDART_INF_F, 0.f);
-            last = -1;
-            if (r >= a.R) return;
-            const float l = __ldg(a.l + (size_t)b * a.R + r);
-            if (l <= 0.f) return;
-            ml = make_float2(__ldg(a.m + (size_t)b * a.R + r) * 1.4426950408889634f, 1.f / l);
-            last = a.causal ? r % a.Sq + n - a.Sq : n - 1;
+        // thread L fetches m and l of rows L and L + 128 of the tile of query rows that starts at r0 (nobody waits for the loads
+        // here) ...
+        struct Stats { float m[2], l[2]; };
+        auto fetch = [&](int b, int r0, Stats &st) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const size_t r = (size_t)b * a.R + min(r0 + L + 128 * i, a.R - 1);
+                st.m[i] = __ldg(a.m + r);
+                st.l[i] = __ldg(a.l + r);
+            }
+        };
+        // ... and keeps, in shared memory, m log2(e), 1 / l and the last key the row sees.  A row that sees nothing gets (inf, 0):
+        // every exponential is 0.
+        auto keep = [&](int buf, int n, int r0, const Stats &st) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int c = L + 128 * i, r = r0 + c;
+                const bool seen = r < a.R && !(st.l[i] <= 0.f);
+                sh.ml[buf][c] = seen ? make_float2(st.m[i] * 1.4426950408889634f, 1.f / st.l[i]) : make_float2(CUDART_INF_F, 0.f);
+                sh.last[buf][c] = !seen ? -1 : (a.causal ? r % a.Sq + n - a.Sq : n - 1);
+            }
         };
         // sum over the columns 0 .. cols - 1 of an accumulator
         auto sum_tile = [&](int acc, int buf, int cols, int t, bool masked) {
@@ -315,14 +340,14 @@ accumulate_kernel(const TcProblem p, const __grid_constant__ CUtensorMap tmQ, co
 #pragma unroll
                     for (int j = 0; j < 32; j += 2) {
                         const float4 q = *reinterpret_cast<const float4 *>(&sh.ml[buf][c + j]);
-                        g0 = fmaf(exp2f(fmaf(__uint_as_float(v[j]), a.scale_log2, -q.x)), q.y, g0);
-                        g1 = fmaf(exp2f(fmaf(__uint_as_float(v[j + 1]), a.scale_log2, -q.z)), q.w, g1);
+                        g0 = fmaf(ex2(fmaf(__uint_as_float(v[j]), a.scale_log2, -q.x)), q.y, g0);
+                        g1 = fmaf(ex2(fmaf(__uint_as_float(v[j + 1]), a.scale_log2, -q.z)), q.w, g1);
                     }
                 } else {
 #pragma unroll
                     for (int j = 0; j < 32; ++j) {
                         const float2 q = sh.ml[buf][c + j];
-                        const float e = exp2f(fmaf(__uint_as_float(v[j]), a.scale_log2, -q.x)) * q.y;
+                        const float e = ex2(fmaf(__uint_as_float(v[j]), a.scale_log2, -q.x)) * q.y;
                         if (c + j < cols && t <= sh.last[buf][c + j]) g0 += e;
                     }
                 }
@@ -334,8 +359,7 @@ accumulate_kernel(const TcProblem p, const __grid_constant__ CUtensorMap tmQ, co
             named_bar_sync(1, 128);
             if (L == 0) mbar_arrive_cluster_relaxed(acc_empty_lead + 8u * acc);
         };
-        auto add = [&](int b, int t, float g) {
-            const long long row = a.pg.row(b, t);
+        auto add = [&](long long row, float g) {
             if (row >= 0) atomicAdd(a.weights + row, g);       // one addition per key; atomic in case sequences share a page
         };
         int buf = 0;
@@ -343,40 +367,38 @@ accumulate_kernel(const TcProblem p, const __grid_constant__ CUtensorMap tmQ, co
         while (!dead && w.next(units)) {
             const int b = w.b, n = w.n;
             if (!ROWS) {
-                float2 ml;
-                int last;
-                fetch(b, n, 0, ml, last);
+                Stats ml;
+                fetch(b, 0, ml);
                 buf ^= 1;
-                sh.ml[buf][L] = ml;
-                sh.last[buf][L] = last;
+                keep(buf, n, 0, ml);
                 named_bar_sync(1, 128);
                 for (int i = 0; i < w.count; ++i) {
                     const int acc = n_done & 1, t = w.t0 + i * KEYS + rank * 128 + L;
+                    const long long row = t < n ? a.pg.row(b, t) : -1;           // under the tile's copies and MMAs
                     ok = __all_sync(0xffffffffu, ok && mbar_wait(ACC_FULL(acc), (n_done >> 1) & 1));
                     tc_fence_after_sync();
                     ++n_done;
                     float g = 0.f;
                     if (ok) g = sum_tile(acc, buf, a.R, t, a.causal && w.t0 + (i + 1) * KEYS > n - a.Sq + 1);
                     release(acc);
-                    if (ok && t < n) add(b, t, g);
+                    if (ok) add(row, g);
                 }
             } else {
-                float2 ml;
-                int last, i = 0;
+                Stats ml;
+                int i = 0;
                 auto skip = [&]() { while (i < w.count && !w.sees(w.r_lo + i)) ++i; };
                 skip();
-                if (i < w.count) fetch(b, n, (w.r_lo + i) * QROWS, ml, last);
+                if (i < w.count) fetch(b, (w.r_lo + i) * QROWS, ml);
                 const int t = w.t0 + rank * 128 + L;
                 float g = 0.f;
                 while (i < w.count) {
                     const int r = w.r_lo + i, acc = n_done & 1;
                     buf ^= 1;                                                    // the other buffer's readers passed a barrier since
-                    sh.ml[buf][L] = ml;
-                    sh.last[buf][L] = last;
+                    keep(buf, n, r * QROWS, ml);
                     named_bar_sync(1, 128);
                     ++i;
                     skip();
-                    if (i < w.count) fetch(b, n, (w.r_lo + i) * QROWS, ml, last);            // under this tile's arithmetic
+                    if (i < w.count) fetch(b, (w.r_lo + i) * QROWS, ml);         // under this tile's arithmetic
                     ok = __all_sync(0xffffffffu, ok && mbar_wait(ACC_FULL(acc), (n_done >> 1) & 1));
                     tc_fence_after_sync();
                     ++n_done;
@@ -384,7 +406,7 @@ accumulate_kernel(const TcProblem p, const __grid_constant__ CUtensorMap tmQ, co
                     release(acc);
                 }
                 if (!ok || t >= n) continue;
-                if (p.splits == 1) add(b, t, g);
+                if (p.splits == 1) add(a.pg.row(b, t), g);
                 else p.partial[((size_t)w.split * a.B + b) * ((size_t)a.pg.max_pages * a.pg.page_size) + t] = g;
             }
         }
