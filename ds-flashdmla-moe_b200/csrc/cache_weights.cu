@@ -118,7 +118,9 @@ __global__ void __launch_bounds__(128) stamp_kernel(float *__restrict__ weights,
 // ---- evict, part 1: which rows stay ------------------------------------------------------------------------------------------
 // One cluster per sequence; CTA r holds the sort keys of its contiguous share of the rows in shared memory, read once.  The
 // keep-th largest key comes from three rounds of 11-, 11- and 10-bit histograms summed over the cluster; the ranks of equal
-// keys, evicted rows and moving rows from counts per warp (a warp owns a contiguous share of its CTA's rows).
+// keys, evicted rows and moving rows from counts per warp (a warp owns a contiguous share of its CTA's rows).  A barrier of 16
+// CTAs costs about 2 us, so there are five: a histogram of its own for every round (nobody waits before clearing one), the
+// counts of equal keys from the last round's, evicted and moving rows counted together.
 constexpr int SEL_THREADS = 1024, SEL_WARPS = SEL_THREADS / 32, BINS = 2048, MAX_CLUSTER = 16;
 constexpr int MAX_SEG = 49152;                   // rows per CTA: 192 KB of keys
 
@@ -145,39 +147,38 @@ __device__ __forceinline__ void cluster_barrier(int cs) {
 }
 
 struct SelShared {
-    uint32_t hist[BINS], total[BINS];
+    alignas(8) uint32_t hist[3][BINS];
     uint32_t warp_n[3][SEL_WARPS + 1];           // per warp: equal keys, evicted rows, moving rows; then their prefix sums
     uint32_t cta_n[3];                           // of the whole CTA, read by the others
     uint32_t base[3];                            // of the CTAs before this one
-    uint32_t scan[SEL_WARPS], prefix, remaining, digit;
+    uint32_t scan[SEL_WARPS], prefix, remaining;
 };
 
-// exclusive prefix sums over the CTA's warps and over the CTAs of the cluster of count `c` (already in sh.warp_n[c])
-__device__ __forceinline__ void ranks(SelShared &sh, int c, int rank, int cs) {
-    __syncthreads();
-    if (threadIdx.x < 32) {
-        const uint32_t v = sh.warp_n[c][threadIdx.x];
-        uint32_t incl = v;
+// count `c` per warp (in sh.warp_n[c]) -> exclusive prefix sums over the CTA's warps, and the CTA's total
+__device__ __forceinline__ void warp_ranks(SelShared &sh, int c) {
+    const int lane = threadIdx.x & 31;
+    const uint32_t v = sh.warp_n[c][lane];
+    uint32_t incl = v;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const uint32_t u = __shfl_up_sync(0xffffffffu, incl, o);
-            if ((int)threadIdx.x >= o) incl += u;
-        }
-        sh.warp_n[c][threadIdx.x] = incl - v;
-        if (threadIdx.x == 31) sh.cta_n[c] = incl;
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t u = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += u;
     }
-    cluster_barrier(cs);
-    if (threadIdx.x == 0) {
-        uint32_t base = 0;
-        for (int r = 0; r < rank; ++r) base += ptx::ld_shared_cluster_u32(ptx::map_to_cta(ptx::smem_u32(&sh.cta_n[c]), r));
-        sh.base[c] = base;
-    }
-    __syncthreads();
+    sh.warp_n[c][lane] = incl - v;
+    if (lane == 31) sh.cta_n[c] = incl;
+}
+// by one warp: sum of *word over the CTAs in front of this one
+__device__ __forceinline__ uint32_t before_cta(const uint32_t *word, int rank) {
+    const int lane = threadIdx.x & 31;
+    uint32_t n = 0;
+    if (lane < rank) n = ptx::ld_shared_cluster_u32(ptx::map_to_cta(ptx::smem_u32(word), lane));
+    return __reduce_add_sync(0xffffffffu, n);
 }
 
 __global__ void __launch_bounds__(SEL_THREADS, 1) select_kernel(const SelectProblem p, const int cs) {
     extern __shared__ uint32_t s_key[];
     __shared__ SelShared sh;
+    ptx::launch_dependents();
     const int rank = cs > 1 ? (int)ptx::cluster_ctarank() : 0, b = blockIdx.x / cs;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int n = p.pg.length(b);
@@ -191,35 +192,59 @@ __global__ void __launch_bounds__(SEL_THREADS, 1) select_kernel(const SelectProb
 
     const int lo = rank * p.seg < n ? rank * p.seg : n, hi = lo + p.seg < n ? lo + p.seg : n, rows = hi - lo;
     const int newest = p.next[b] - p.recent;
-    for (int i = tid; i < rows; i += SEL_THREADS) {
-        const long long row = p.pg.row(b, lo + i);
-        uint32_t key = 0u;
-        if (row >= 0) key = p.positions[row] >= newest ? 0xffffffffu : sort_key(p.weights[row]);
-        s_key[i] = key;
+    // four rows a thread at a time: first their pages, then positions and weights, so that three latencies serve four rows
+    const int32_t *table = p.pg.table + (size_t)b * p.pg.max_pages;
+    for (int i0 = tid; i0 < rows; i0 += 4 * SEL_THREADS) {
+        int pg[4], in_page[4], pos[4];
+        float wt[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int t = lo + min(i0 + j * SEL_THREADS, rows - 1), lp = t / p.pg.page_size;
+            pg[j] = __ldg(table + lp);
+            in_page[j] = t - lp * p.pg.page_size;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (pg[j] < 0 || pg[j] >= p.pg.num_pages) { g_cache_error = ERR_PAGE; pg[j] = -1; }
+            const size_t row = (size_t)max(pg[j], 0) * p.pg.page_size + in_page[j];
+            pos[j] = pg[j] >= 0 ? __ldcg(p.positions + row) : 0;
+            wt[j] = pg[j] >= 0 ? __ldcg(p.weights + row) : 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int i = i0 + j * SEL_THREADS;
+            if (i < rows) s_key[i] = pg[j] < 0 ? 0u : (pos[j] >= newest ? 0xffffffffu : sort_key(wt[j]));
+        }
     }
     if (tid == 0) { sh.prefix = 0u; sh.remaining = (uint32_t)K; }
+    for (int i = tid; i < 3 * BINS; i += SEL_THREADS) (&sh.hist[0][0])[i] = 0u;
 
     // the K-th largest key, from the top digit down
     for (int round = 0; round < 3; ++round) {
         const int shift = round == 0 ? 21 : (round == 1 ? 10 : 0), bits = round == 2 ? 10 : 11, bins = 1 << bits;
-        for (int i = tid; i < BINS; i += SEL_THREADS) sh.hist[i] = 0u;
+        uint32_t *hist = sh.hist[round];
         __syncthreads();
-        const uint32_t prefix = sh.prefix;
+        const uint32_t prefix = sh.prefix, want = sh.remaining;
         for (int i = tid; i < rows; i += SEL_THREADS) {
             const uint32_t key = s_key[i];
-            if (round == 0 || (key >> (shift + bits)) == prefix) atomicAdd(&sh.hist[(key >> shift) & (bins - 1)], 1u);
+            if (round == 0 || (key >> (shift + bits)) == prefix) atomicAdd(&hist[(key >> shift) & (bins - 1)], 1u);
         }
         cluster_barrier(cs);                     // every CTA's histogram stands
-        for (int i = tid; i < bins; i += SEL_THREADS) {
-            uint32_t v = 0;
-            if (cs == 1) v = sh.hist[i];
-            else for (int r = 0; r < cs; ++r) v += ptx::ld_shared_cluster_u32(ptx::map_to_cta(ptx::smem_u32(&sh.hist[i]), r));
-            sh.total[i] = v;
-        }
-        __syncthreads();
-        // thread i owns the two bins from the top; the digit is where the running count reaches what is still to be taken
+        // thread i owns two bins, from the top; the digit is where the running count reaches what is still to be taken
         const int hi_bin = bins - 1 - 2 * tid;
-        const uint32_t c0 = hi_bin >= 1 ? sh.total[hi_bin] : 0u, c1 = hi_bin >= 1 ? sh.total[hi_bin - 1] : 0u;
+        uint32_t c0 = 0, c1 = 0;
+        if (hi_bin >= 1) {
+            if (cs == 1) { c0 = hist[hi_bin]; c1 = hist[hi_bin - 1]; }
+            else
+                for (int r0 = 0; r0 < cs; r0 += 8) {             // the CTAs' counts, eight loads in flight
+                    uint2 v[8];
+#pragma unroll
+                    for (int r = 0; r < 8; ++r)
+                        v[r] = r0 + r < cs ? ptx::ld_shared_cluster_v2(ptx::map_to_cta(ptx::smem_u32(&hist[hi_bin - 1]), r0 + r)) : make_uint2(0u, 0u);
+#pragma unroll
+                    for (int r = 0; r < 8; ++r) { c1 += v[r].x; c0 += v[r].y; }
+                }
+        }
         uint32_t incl = c0 + c1;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -228,16 +253,15 @@ __global__ void __launch_bounds__(SEL_THREADS, 1) select_kernel(const SelectProb
         }
         if (lane == 31) sh.scan[warp] = incl;
         __syncthreads();
-        for (int w = 0; w < warp; ++w) incl += sh.scan[w];
-        const uint32_t before = incl - c0 - c1, want = sh.remaining;
-        __syncthreads();
+        incl += __reduce_add_sync(0xffffffffu, lane < warp ? sh.scan[lane] : 0u);
+        const uint32_t before = incl - c0 - c1;
         if (before < want && want <= incl) {     // exactly one thread
             const bool first = before + c0 >= want;
             sh.prefix = (prefix << bits) | (uint32_t)(first ? hi_bin : hi_bin - 1);
             sh.remaining = want - before - (first ? 0u : c0);
         }
-        cluster_barrier(cs);                     // nobody clears a histogram that is still being read
     }
+    __syncthreads();
     const uint32_t T = sh.prefix, take = sh.remaining;       // of the keys equal to T the first `take` rows stay
 
     // a warp owns rows [wlo, whi) of the CTA
@@ -247,7 +271,13 @@ __global__ void __launch_bounds__(SEL_THREADS, 1) select_kernel(const SelectProb
     for (int i = wlo + lane; i < whi; i += 32) cnt += s_key[i] == T;
     cnt = __reduce_add_sync(0xffffffffu, cnt);
     if (lane == 0) sh.warp_n[0][warp] = cnt;
-    ranks(sh, 0, rank, cs);
+    __syncthreads();
+    if (warp == 0) warp_ranks(sh, 0);
+    if (warp == 1) {                             // a CTA's keys equal to T: its count in the last round's histogram
+        const uint32_t n = before_cta(&sh.hist[2][T & 1023u], rank);
+        if (lane == 0) sh.base[0] = n;
+    }
+    __syncthreads();
     const uint32_t eq0 = sh.base[0] + sh.warp_n[0][warp];
     const uint32_t below = (1u << lane) - 1u;
     for (int pass = 0; pass < 3; ++pass) {       // 0: count, 1: movers write their rows, 2: evicted rows take them
@@ -270,54 +300,74 @@ __global__ void __launch_bounds__(SEL_THREADS, 1) select_kernel(const SelectProb
         }
         if (pass == 0) {
             if (lane == 0) { sh.warp_n[1][warp] = holes; sh.warp_n[2][warp] = moves; }
-            ranks(sh, 1, rank, cs);
-            ranks(sh, 2, rank, cs);
+            __syncthreads();
+            if (warp < 2) warp_ranks(sh, 1 + warp);
+            cluster_barrier(cs);
+            if (warp < 2) {
+                const uint32_t n = before_cta(&sh.cta_n[1 + warp], rank);
+                if (lane == 0) sh.base[1 + warp] = n;
+            }
+            __syncthreads();
         } else if (pass == 1) {
             __threadfence();
-            cluster_barrier(cs);                 // the list of movers stands; also: nobody leaves while its counts are read
+            cluster_barrier(cs);                 // the list of movers stands; nobody leaves while its counts are read
         }
     }
     if (rank == 0 && tid == 0) p.new_lens[b] = K;            // last: it may be the array the lengths were read from
 }
 
 // ---- evict, part 2: the copies -----------------------------------------------------------------------------------------------
-// A warp takes 32 places j at a time, reads what goes there (kept) and copies the rows that change place, two at a time.
+// A warp takes `span` places (up to 32, fewer when there are few), reads what goes there (kept) and copies the rows that change
+// place, two at a time with three vectors of each in flight per lane (a row of 1152 bytes is 72 vectors of 16; four rows at a
+// time take more registers and were 5 % slower).  Rows are read and written once: streaming loads and stores.
 template <typename V>
 __global__ void __launch_bounds__(256) move_kernel(uint8_t *__restrict__ pool, float *__restrict__ weights,
-                                                   int32_t *__restrict__ positions, const int32_t *__restrict__ kept, const Pages pg,
-                                                   int B, int keep, int row_bytes) {
+                                                   int32_t *__restrict__ positions, const int32_t *kept, const Pages pg, int B, int keep,
+                                                   int row_bytes, int span) {
+    ptx::wait_for_primary();                     // kept is the select kernel's
     const int lane = threadIdx.x & 31;
-    const int groups = (keep + 31) / 32;
+    const int groups = (keep + span - 1) / span;
     const long long warps = (long long)gridDim.x * 8;
     const int vecs = row_bytes / (int)sizeof(V);
     for (long long g = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); g < (long long)B * groups; g += warps) {
-        const int b = (int)(g / groups), j = (int)(g - (long long)b * groups) * 32 + lane;
-        const int src = j < keep ? kept[(size_t)b * keep + j] : -1;
+        const int b = (int)(g / groups), j = (int)(g - (long long)b * groups) * span + lane;
+        const int src = lane < span && j < keep ? __ldcg(kept + (size_t)b * keep + j) : -1;
         long long from = -1, to = -1;
         if (src >= 0 && src != j) {
             from = pg.row(b, src);
             to = pg.row(b, j);
         }
         const bool moves = from >= 0 && to >= 0;
+        uint32_t todo = __ballot_sync(0xffffffffu, moves);
+        while (todo) {
+            const V *f[2];
+            V *d[2];
+            int n = 0;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int a = todo ? __ffs(todo) - 1 : 0;
+                const long long fr = __shfl_sync(0xffffffffu, from, a), tt = __shfl_sync(0xffffffffu, to, a);
+                if (todo) { f[i] = reinterpret_cast<const V *>(pool + fr * row_bytes); d[i] = reinterpret_cast<V *>(pool + tt * row_bytes); ++n; }
+                else { f[i] = f[0]; d[i] = d[0]; }
+                todo &= todo - 1;
+            }
+            for (int v0 = lane; v0 < vecs; v0 += 96) {
+                V x[2][3];
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int q = 0; q < 3; ++q)
+                        if (i < n && v0 + 32 * q < vecs) x[i][q] = __ldcs(f[i] + v0 + 32 * q);
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int q = 0; q < 3; ++q)
+                        if (i < n && v0 + 32 * q < vecs) __stcs(d[i] + v0 + 32 * q, x[i][q]);
+            }
+        }
         if (moves) {
             weights[to] = weights[from];
             positions[to] = positions[from];
-        }
-        uint32_t todo = __ballot_sync(0xffffffffu, moves);
-        while (todo) {
-            const int a = __ffs(todo) - 1;
-            todo &= todo - 1;
-            const int c = todo ? __ffs(todo) - 1 : a;
-            todo &= todo ? todo - 1 : 0u;
-            const V *f0 = reinterpret_cast<const V *>(pool + __shfl_sync(0xffffffffu, from, a) * row_bytes);
-            const V *f1 = reinterpret_cast<const V *>(pool + __shfl_sync(0xffffffffu, from, c) * row_bytes);
-            V *d0 = reinterpret_cast<V *>(pool + __shfl_sync(0xffffffffu, to, a) * row_bytes);
-            V *d1 = reinterpret_cast<V *>(pool + __shfl_sync(0xffffffffu, to, c) * row_bytes);
-            for (int v = lane; v < vecs; v += 32) {
-                const V x = f0[v], y = f1[v];
-                d0[v] = x;
-                if (c != a) d1[v] = y;
-            }
         }
     }
 }
@@ -452,14 +502,29 @@ extern "C" int fdmla_cache_evict(void *kv_pool, float *weights, int32_t *positio
     if (cudaLaunchKernelEx(&cfg, cw::select_kernel, p, cs) != cudaSuccess) { cudaGetLastError(); return FDMLA_ERR_CUDA; }
     if (cap <= keep) return check_launch();                   // no sequence can be over its bound
     const int row_bytes = d_qk * (dtype == FDMLA_F32 ? 4 : 2);
-    const long long warps = (long long)B * ((keep + 31) / 32);
+    // a warp per `span` places: few rows are spread over the SMs
+    int span = 32;
+    while (span > 4 && (long long)B * ((keep + span - 1) / span) < 4LL * 8 * kNumSMs) span /= 2;
+    const long long warps = (long long)B * ((keep + span - 1) / span);
     const unsigned blocks = (unsigned)(warps > 8LL * 8 * kNumSMs ? 8 * kNumSMs : (warps + 7) / 8);
+    cudaLaunchAttribute pdl;
+    pdl.id = cudaLaunchAttributeProgrammaticStreamSerialization;       // set up while the select kernel runs
+    pdl.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t mv{};
+    mv.gridDim = dim3(blocks);
+    mv.blockDim = dim3(256);
+    mv.stream = s;
+    mv.attrs = &pdl;
+    mv.numAttrs = 1;
     uint8_t *pool = static_cast<uint8_t *>(kv_pool);
+    const int32_t *k = kept;
+    cudaError_t e;
     if (row_bytes % 16 == 0 && (reinterpret_cast<uintptr_t>(kv_pool) & 15) == 0)
-        cw::move_kernel<uint4><<<blocks, 256, 0, s>>>(pool, weights, positions, kept, p.pg, B, keep, row_bytes);
+        e = cudaLaunchKernelEx(&mv, cw::move_kernel<uint4>, pool, weights, positions, k, p.pg, B, keep, row_bytes, span);
     else if (row_bytes % 4 == 0)
-        cw::move_kernel<uint32_t><<<blocks, 256, 0, s>>>(pool, weights, positions, kept, p.pg, B, keep, row_bytes);
+        e = cudaLaunchKernelEx(&mv, cw::move_kernel<unsigned int>, pool, weights, positions, k, p.pg, B, keep, row_bytes, span);
     else
-        cw::move_kernel<uint16_t><<<blocks, 256, 0, s>>>(pool, weights, positions, kept, p.pg, B, keep, row_bytes);
+        e = cudaLaunchKernelEx(&mv, cw::move_kernel<unsigned short>, pool, weights, positions, k, p.pg, B, keep, row_bytes, span);
+    if (e != cudaSuccess) { cudaGetLastError(); return FDMLA_ERR_CUDA; }
     return check_launch();
 }
