@@ -119,8 +119,9 @@ __global__ void __launch_bounds__(128) stamp_kernel(float *__restrict__ weights,
 // One cluster per sequence; CTA r holds the sort keys of its contiguous share of the rows in shared memory, read once.  The
 // keep-th largest key comes from three rounds of 11-, 11- and 10-bit histograms summed over the cluster; the ranks of equal
 // keys, evicted rows and moving rows from counts per warp (a warp owns a contiguous share of its CTA's rows).  A barrier of 16
-// CTAs costs about 2 us, so there are five: a histogram of its own for every round (nobody waits before clearing one), the
-// counts of equal keys from the last round's, evicted and moving rows counted together.
+// CTAs costs about 1 us, so there are five: a histogram of its own for every round (nobody waits before clearing one), the
+// counts of equal keys from the last round's, evicted and moving rows counted together.  Reading all 2048 bins of 16 CTAs took
+// 6 us a round; now every CTA reads their 64 sums of 32 bins, then the 32 bins of the one that matters: 131072 rows 40 -> 23 us.
 constexpr int SEL_THREADS = 1024, SEL_WARPS = SEL_THREADS / 32, BINS = 2048, MAX_CLUSTER = 16;
 constexpr int MAX_SEG = 49152;                   // rows per CTA: 192 KB of keys
 
@@ -131,8 +132,8 @@ struct SelectProblem {
     const int32_t *next;                         // [B] position of the next row to come
     int32_t *kept;                               // [B, keep]: the row that row j held before, -1 past the end
     int32_t *new_lens;                           // [B]
-    int32_t *movers;                             // [B, mover_cap] scratch: rows that move, in order
-    int keep, recent, seg, mover_cap;
+    int32_t *movers, *holes;                     // [B, cap] scratch each: rows that move and evicted rows they replace, in order
+    int keep, recent, seg, cap;
 };
 
 __device__ __forceinline__ uint32_t sort_key(float w) {
@@ -147,32 +148,37 @@ __device__ __forceinline__ void cluster_barrier(int cs) {
 }
 
 struct SelShared {
-    alignas(8) uint32_t hist[3][BINS];
+    uint32_t hist[3][BINS], coarse[3][BINS / 32];
+    uint32_t part[MAX_CLUSTER][BINS / 32];
     uint32_t warp_n[3][SEL_WARPS + 1];           // per warp: equal keys, evicted rows, moving rows; then their prefix sums
     uint32_t cta_n[3];                           // of the whole CTA, read by the others
     uint32_t base[3];                            // of the CTAs before this one
-    uint32_t scan[SEL_WARPS], prefix, remaining;
+    uint32_t total[3];                           // of the whole cluster
+    uint32_t scan[SEL_WARPS], prefix, remaining, group;
 };
 
+__device__ __forceinline__ uint32_t warp_scan(uint32_t v) {              // inclusive, over the lanes
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t u = __shfl_up_sync(0xffffffffu, v, o);
+        if ((threadIdx.x & 31) >= o) v += u;
+    }
+    return v;
+}
 // count `c` per warp (in sh.warp_n[c]) -> exclusive prefix sums over the CTA's warps, and the CTA's total
 __device__ __forceinline__ void warp_ranks(SelShared &sh, int c) {
     const int lane = threadIdx.x & 31;
     const uint32_t v = sh.warp_n[c][lane];
-    uint32_t incl = v;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t u = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += u;
-    }
+    const uint32_t incl = warp_scan(v);
     sh.warp_n[c][lane] = incl - v;
     if (lane == 31) sh.cta_n[c] = incl;
 }
-// by one warp: sum of *word over the CTAs in front of this one
-__device__ __forceinline__ uint32_t before_cta(const uint32_t *word, int rank) {
+// by one warp: sum of *word over the first n CTAs of the cluster
+__device__ __forceinline__ uint32_t sum_ctas(const uint32_t *word, int n) {
     const int lane = threadIdx.x & 31;
-    uint32_t n = 0;
-    if (lane < rank) n = ptx::ld_shared_cluster_u32(ptx::map_to_cta(ptx::smem_u32(word), lane));
-    return __reduce_add_sync(0xffffffffu, n);
+    uint32_t v = 0;
+    if (lane < n) v = ptx::ld_shared_cluster_u32(ptx::map_to_cta(ptx::smem_u32(word), lane));
+    return __reduce_add_sync(0xffffffffu, v);
 }
 
 __global__ void __launch_bounds__(SEL_THREADS, 1) select_kernel(const SelectProblem p, const int cs) {
@@ -229,36 +235,62 @@ __global__ void __launch_bounds__(SEL_THREADS, 1) select_kernel(const SelectProb
             const uint32_t key = s_key[i];
             if (round == 0 || (key >> (shift + bits)) == prefix) atomicAdd(&hist[(key >> shift) & (bins - 1)], 1u);
         }
-        cluster_barrier(cs);                     // every CTA's histogram stands
-        // thread i owns two bins, from the top; the digit is where the running count reaches what is still to be taken
-        const int hi_bin = bins - 1 - 2 * tid;
-        uint32_t c0 = 0, c1 = 0;
-        if (hi_bin >= 1) {
-            if (cs == 1) { c0 = hist[hi_bin]; c1 = hist[hi_bin - 1]; }
-            else
-                for (int r0 = 0; r0 < cs; r0 += 8) {             // the CTAs' counts, eight loads in flight
-                    uint2 v[8];
-#pragma unroll
-                    for (int r = 0; r < 8; ++r)
-                        v[r] = r0 + r < cs ? ptx::ld_shared_cluster_v2(ptx::map_to_cta(ptx::smem_u32(&hist[hi_bin - 1]), r0 + r)) : make_uint2(0u, 0u);
-#pragma unroll
-                    for (int r = 0; r < 8; ++r) { c1 += v[r].x; c0 += v[r].y; }
-                }
+        if (cs == 1) {
+            __syncthreads();
+            // thread i owns two bins, from the top; the digit is where the running count reaches what is still to be taken
+            const int hi_bin = bins - 1 - 2 * tid;
+            const uint32_t c0 = hi_bin >= 1 ? hist[hi_bin] : 0u, c1 = hi_bin >= 1 ? hist[hi_bin - 1] : 0u;
+            uint32_t incl = warp_scan(c0 + c1);
+            if (lane == 31) sh.scan[warp] = incl;
+            __syncthreads();
+            incl += __reduce_add_sync(0xffffffffu, lane < warp ? sh.scan[lane] : 0u);
+            const uint32_t before = incl - c0 - c1;
+            if (before < want && want <= incl) {     // exactly one thread
+                const bool first = before + c0 >= want;
+                sh.prefix = (prefix << bits) | (uint32_t)(first ? hi_bin : hi_bin - 1);
+                sh.remaining = want - before - (first ? 0u : c0);
+            }
+            continue;
         }
-        uint32_t incl = c0 + c1;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const uint32_t u = __shfl_up_sync(0xffffffffu, incl, o);
-            if (lane >= o) incl += u;
-        }
-        if (lane == 31) sh.scan[warp] = incl;
+        // sums of 32 bins
         __syncthreads();
-        incl += __reduce_add_sync(0xffffffffu, lane < warp ? sh.scan[lane] : 0u);
-        const uint32_t before = incl - c0 - c1;
-        if (before < want && want <= incl) {     // exactly one thread
-            const bool first = before + c0 >= want;
-            sh.prefix = (prefix << bits) | (uint32_t)(first ? hi_bin : hi_bin - 1);
-            sh.remaining = want - before - (first ? 0u : c0);
+        const int groups = bins / 32;
+        for (int g = warp; g < groups; g += SEL_WARPS) {
+            const uint32_t n = __reduce_add_sync(0xffffffffu, hist[g * 32 + lane]);
+            if (lane == 0) sh.coarse[round][g] = n;
+        }
+        cluster_barrier(cs);                     // every CTA's histogram stands
+        {   // a thread per CTA and group
+            const int r = tid >> 6, g = tid & 63;
+            sh.part[r][g] = r < cs && g < groups ? ptx::ld_shared_cluster_u32(ptx::map_to_cta(ptx::smem_u32(&sh.coarse[round][g]), r)) : 0u;
+        }
+        __syncthreads();
+        if (warp == 0) {                         // lane i owns the groups 63 - 2 i and 62 - 2 i
+            uint32_t c0 = 0, c1 = 0;
+            for (int r = 0; r < cs; ++r) { c0 += sh.part[r][63 - 2 * lane]; c1 += sh.part[r][62 - 2 * lane]; }
+            const uint32_t incl = warp_scan(c0 + c1), before = incl - c0 - c1;
+            if (before < want && want <= incl) {
+                const bool first = before + c0 >= want;
+                sh.group = 63 - 2 * lane - (first ? 0 : 1);
+                sh.remaining = want - before - (first ? 0u : c0);
+            }
+        }
+        __syncthreads();
+        const uint32_t group = sh.group;
+        if (tid < 32 * MAX_CLUSTER) {            // a thread per CTA and bin of the group
+            const int r = tid >> 5;
+            sh.part[r][lane] = r < cs ? ptx::ld_shared_cluster_u32(ptx::map_to_cta(ptx::smem_u32(&hist[group * 32 + lane]), r)) : 0u;
+        }
+        __syncthreads();
+        if (warp == 0) {                         // lane i owns bin 31 - i of the group
+            uint32_t c = 0;
+            for (int r = 0; r < cs; ++r) c += sh.part[r][31 - lane];
+            const uint32_t left = sh.remaining, incl = warp_scan(c);
+            __syncwarp();
+            if (incl - c < left && left <= incl) {
+                sh.prefix = (prefix << bits) | (group * 32 + 31 - lane);
+                sh.remaining = left - (incl - c);
+            }
         }
     }
     __syncthreads();
@@ -274,13 +306,14 @@ __global__ void __launch_bounds__(SEL_THREADS, 1) select_kernel(const SelectProb
     __syncthreads();
     if (warp == 0) warp_ranks(sh, 0);
     if (warp == 1) {                             // a CTA's keys equal to T: its count in the last round's histogram
-        const uint32_t n = before_cta(&sh.hist[2][T & 1023u], rank);
+        const uint32_t n = sum_ctas(&sh.hist[2][T & 1023u], rank);
         if (lane == 0) sh.base[0] = n;
     }
     __syncthreads();
     const uint32_t eq0 = sh.base[0] + sh.warp_n[0][warp];
     const uint32_t below = (1u << lane) - 1u;
-    for (int pass = 0; pass < 3; ++pass) {       // 0: count, 1: movers write their rows, 2: evicted rows take them
+    int32_t *movers = p.movers + (size_t)b * p.cap, *holes_at = p.holes + (size_t)b * p.cap;
+    for (int pass = 0; pass < 2; ++pass) {       // 0: count, 1: list
         uint32_t eq = eq0;
         uint32_t holes = 0, moves = 0;
         if (pass > 0) { holes = sh.base[1] + sh.warp_n[1][warp]; moves = sh.base[2] + sh.warp_n[2][warp]; }
@@ -292,8 +325,8 @@ __global__ void __launch_bounds__(SEL_THREADS, 1) select_kernel(const SelectProb
             const bool stays = live && (key > T || (key == T && eq + __popc(eqs & below) < take));
             const uint32_t hole = __ballot_sync(0xffffffffu, live && t < K && !stays);
             const uint32_t move = __ballot_sync(0xffffffffu, live && t >= K && stays);
-            if (pass == 1 && ((move >> lane) & 1u)) p.movers[(size_t)b * p.mover_cap + moves + __popc(move & below)] = t;
-            if (pass == 2 && ((hole >> lane) & 1u)) kept[t] = __ldcg(p.movers + (size_t)b * p.mover_cap + holes + __popc(hole & below));
+            if (pass == 1 && ((move >> lane) & 1u)) movers[moves + __popc(move & below)] = t;
+            if (pass == 1 && ((hole >> lane) & 1u)) holes_at[holes + __popc(hole & below)] = t;
             eq += __popc(eqs);
             holes += __popc(hole);
             moves += __popc(move);
@@ -304,15 +337,15 @@ __global__ void __launch_bounds__(SEL_THREADS, 1) select_kernel(const SelectProb
             if (warp < 2) warp_ranks(sh, 1 + warp);
             cluster_barrier(cs);
             if (warp < 2) {
-                const uint32_t n = before_cta(&sh.cta_n[1 + warp], rank);
-                if (lane == 0) sh.base[1 + warp] = n;
+                const uint32_t n = sum_ctas(&sh.cta_n[1 + warp], rank), all = sum_ctas(&sh.cta_n[1 + warp], cs);
+                if (lane == 0) { sh.base[1 + warp] = n; sh.total[1 + warp] = all; }
             }
             __syncthreads();
-        } else if (pass == 1) {
-            __threadfence();
-            cluster_barrier(cs);                 // the list of movers stands; nobody leaves while its counts are read
         }
     }
+    __threadfence();
+    cluster_barrier(cs);                         // the lists stand; nobody leaves while its counts are read
+    for (uint32_t r = rank * SEL_THREADS + tid; r < sh.total[1]; r += cs * SEL_THREADS) kept[__ldcg(holes_at + r)] = __ldcg(movers + r);
     if (rank == 0 && tid == 0) p.new_lens[b] = K;            // last: it may be the array the lengths were read from
 }
 
@@ -458,7 +491,7 @@ extern "C" int fdmla_cache_stamp(float *weights, int32_t *positions, const int32
 extern "C" size_t fdmla_cache_evict_workspace_bytes(int B, int keep, int page_size, int max_pages) {
     if (B <= 0 || keep <= 0 || page_size <= 0 || max_pages <= 0) return 0;
     const long long cap = (long long)page_size * max_pages, movers = keep < cap ? keep : cap;
-    return (size_t)B * movers * sizeof(int32_t);
+    return (size_t)2 * B * movers * sizeof(int32_t);
 }
 
 extern "C" int fdmla_cache_evict(void *kv_pool, float *weights, int32_t *positions, const int32_t *page_table,
@@ -482,7 +515,8 @@ extern "C" int fdmla_cache_evict(void *kv_pool, float *weights, int32_t *positio
     p.weights = weights; p.positions = positions;
     p.pg = cw::Pages{page_table, seqlens, page_size, max_pages, num_pages};
     p.next = next_position; p.kept = kept; p.new_lens = new_seqlens; p.movers = static_cast<int32_t *>(workspace);
-    p.keep = keep; p.recent = recent; p.seg = seg; p.mover_cap = keep < cap ? keep : cap;
+    p.keep = keep; p.recent = recent; p.seg = seg; p.cap = keep < cap ? keep : cap;
+    p.holes = p.movers + (size_t)B * p.cap;
     const size_t smem = (size_t)seg * 4;
     if (cudaFuncSetAttribute(cw::select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, cw::MAX_SEG * 4) != cudaSuccess ||
         (cs > 8 && cudaFuncSetAttribute(cw::select_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)) {

@@ -23,7 +23,7 @@ import torch.distributed as dist
 
 from . import _lib
 from ._lib import FlashDMLAError, check
-from .ops import _dtype_code, _need_cuda, _ptr, _stream
+from .ops import _dtype_code, _launch_on, _need_cuda, _ptr, _stream
 
 
 def route_topk(logits: torch.Tensor, k: int):
@@ -112,35 +112,42 @@ def moe_few(x: torch.Tensor, Wg: torch.Tensor, W1: torch.Tensor, W3: torch.Tenso
     winners' logits; there is no capacity and nothing is dropped.  Every chosen expert's weights are read once.  Weights have
     to be finite.  out: a contiguous tensor to write into."""
     _need_cuda(x, Wg, W1, W3, W2, *(shared or ()))
-    if x.dim() != 2 or Wg.dim() != 2 or W1.dim() != 3 or W2.dim() != 3:
+    if x.dim() != 2 or W1.dim() != 3:
         raise FlashDMLAError("expected x [T,d], Wg [d,E], W1, W3 [E,d,f], W2 [E,f,d]")
-    (T, d), (E, _, f) = x.shape, W1.shape
-    if tuple(Wg.shape) != (d, E) or tuple(W1.shape) != (E, d, f) or W3.shape != W1.shape or tuple(W2.shape) != (E, f, d):
+    (T, d), (E, _, f), dt = x.shape, W1.shape, x.dtype
+    if Wg.shape != (d, E) or W1.shape != (E, d, f) or W3.shape != (E, d, f) or W2.shape != (E, f, d):
         raise FlashDMLAError("shape mismatch between x, Wg, W1, W3 and W2")
     if Wg.dtype != torch.float32:
         raise FlashDMLAError("the gate weights must be float32")
-    if any(t.dtype != x.dtype for t in (W1, W3, W2, *(shared or ()))):
+    if W1.dtype != dt or W3.dtype != dt or W2.dtype != dt:
         raise FlashDMLAError("x and the expert weights must share one dtype")
-    if shared is not None and [tuple(t.shape) for t in shared] != [(d, f), (d, f), (f, d)]:
-        raise FlashDMLAError("the shared expert must be (S1 [d,f], S3 [d,f], S2 [f,d])")
+    s1 = s3 = s2 = None
+    if shared is not None:
+        S1, S3, S2 = shared
+        if S1.shape != (d, f) or S3.shape != (d, f) or S2.shape != (f, d):
+            raise FlashDMLAError("the shared expert must be (S1 [d,f], S3 [d,f], S2 [f,d])")
+        if S1.dtype != dt or S3.dtype != dt or S2.dtype != dt:
+            raise FlashDMLAError("x and the expert weights must share one dtype")
+        S1, S3, S2 = S1.contiguous(), S3.contiguous(), S2.contiguous()
+        s1, s3, s2 = S1.data_ptr(), S3.data_ptr(), S2.data_ptr()
     if T > MAX_FEW_TOKENS:
         raise FlashDMLAError(f"moe_few takes at most {MAX_FEW_TOKENS} tokens, got {T}")
     k = int(k)
     if not 1 <= k <= min(E, 32):
         raise FlashDMLAError("k must be between 1 and min(E, 32)")
-    x, Wg, W1, W3, W2 = (t.contiguous() for t in (x, Wg, W1, W3, W2))
-    S1, S3, S2 = (t.contiguous() for t in shared) if shared is not None else (None, None, None)
-    if out is None:
-        out = torch.empty(T, d, dtype=x.dtype, device=x.device)
-    elif tuple(out.shape) != (T, d) or out.dtype != x.dtype or out.device != x.device or not out.is_contiguous():
-        raise FlashDMLAError("out must be a contiguous [T,d] tensor of x's dtype on its GPU")
+    x, Wg, W1, W3, W2 = x.contiguous(), Wg.contiguous(), W1.contiguous(), W3.contiguous(), W2.contiguous()
     code = _dtype_code(x)
-    with torch.cuda.device(x.device):
+    if out is None:
+        out = torch.empty(T, d, dtype=dt, device=x.device)
+    elif out.shape != (T, d) or out.dtype != dt or out.device != x.device or not out.is_contiguous():
+        raise FlashDMLAError("out must be a contiguous [T,d] tensor of x's dtype on its GPU")
+    ctx, stream = _launch_on(x)
+    with ctx:
         L = _lib.lib()
         nbytes = L.fdmla_moe_few_workspace_bytes(T, d, f, E, k, int(shared is not None), code)
         ws = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=x.device)
-        check(L.fdmla_moe_few(_ptr(x), _ptr(Wg), _ptr(W1), _ptr(W3), _ptr(W2), _ptr(S1), _ptr(S3), _ptr(S2), _ptr(out),
-                              _ptr(ws), ws.numel(), T, d, f, E, k, code, _stream(x)), "fdmla_moe_few")
+        check(L.fdmla_moe_few(x.data_ptr(), Wg.data_ptr(), W1.data_ptr(), W3.data_ptr(), W2.data_ptr(), s1, s3, s2, out.data_ptr(),
+                              ws.data_ptr(), max(nbytes, 256), T, d, f, E, k, code, stream), "fdmla_moe_few")
     return out
 
 

@@ -11,6 +11,7 @@ eager fallback.
 """
 from __future__ import annotations
 
+import contextlib
 import math
 from typing import Optional, Tuple
 
@@ -43,6 +44,18 @@ def _need_cuda(*ts: torch.Tensor) -> None:
 
 def _stream(t: torch.Tensor) -> int:
     return torch.cuda.current_stream(t.device).cuda_stream
+
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_current = contextlib.nullcontext()
+
+
+def _launch_on(t: torch.Tensor):
+    """(context, stream) for a launch on t's GPU.  Where a call takes ten microseconds on the GPU, entering a device that is
+    current already and building a Stream object would take the host half as long."""
+    dev = t.device.index
+    ctx = _current if dev == torch.cuda.current_device() else torch.cuda.device(dev)
+    return ctx, _raw_stream(dev) if _raw_stream is not None else _stream(t)
 
 
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
@@ -435,18 +448,18 @@ def _check_tables(page_table, B, *per_seq) -> None:
     if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != B:
         raise FlashDMLAError("page_table must be [B, max_pages] int32")
     for t in per_seq:
-        if t.dtype != torch.int32 or tuple(t.shape) != (B,):
+        if t.dtype != torch.int32 or t.shape != (B,):
             raise FlashDMLAError("lengths and positions per sequence must be [B] int32")
 
 
 def _check_row_state(kv_pool, weights, positions=None) -> None:
     if kv_pool.dim() != 3 or not kv_pool.is_contiguous():
         raise FlashDMLAError("kv_pool must be a contiguous [num_pages, page_size, d_qk] tensor")
-    for t, dt, name in ((weights, torch.float32, "weights"), (positions, torch.int32, "positions")):
-        if t is None:
-            continue
-        if t.dtype != dt or tuple(t.shape) != tuple(kv_pool.shape[:2]) or not t.is_contiguous():
-            raise FlashDMLAError(f"{name} must be a contiguous [num_pages, page_size] {dt} tensor (it is written in place)")
+    pages = kv_pool.shape[:2]
+    if weights.dtype != torch.float32 or weights.shape != pages or not weights.is_contiguous():
+        raise FlashDMLAError("weights must be a contiguous [num_pages, page_size] float32 tensor (it is written in place)")
+    if positions is not None and (positions.dtype != torch.int32 or positions.shape != pages or not positions.is_contiguous()):
+        raise FlashDMLAError("positions must be a contiguous [num_pages, page_size] int32 tensor (it is written in place)")
 
 
 def cache_stamp(weights, positions, page_table, start_pos, first_position, n_tokens: int) -> None:
@@ -458,11 +471,12 @@ def cache_stamp(weights, positions, page_table, start_pos, first_position, n_tok
             or not weights.is_contiguous() or not positions.is_contiguous():
         raise FlashDMLAError("weights (float32) and positions (int32) must be contiguous [num_pages, page_size] tensors")
     num_pages, page_size = weights.shape
-    with torch.cuda.device(weights.device):
-        check(_lib.lib().fdmla_cache_stamp(_ptr(weights), _ptr(positions), _ptr(page_table.contiguous()),
-                                           _ptr(start_pos.contiguous()), _ptr(first_position.contiguous()), page_table.shape[0],
-                                           int(n_tokens), page_size, page_table.shape[1], num_pages, _stream(weights)),
-              "fdmla_cache_stamp")
+    page_table, start_pos, first_position = page_table.contiguous(), start_pos.contiguous(), first_position.contiguous()
+    ctx, stream = _launch_on(weights)
+    with ctx:
+        check(_lib.lib().fdmla_cache_stamp(weights.data_ptr(), positions.data_ptr(), page_table.data_ptr(), start_pos.data_ptr(),
+                                           first_position.data_ptr(), page_table.shape[0], int(n_tokens), page_size,
+                                           page_table.shape[1], num_pages, stream), "fdmla_cache_stamp")
 
 
 def accumulate_weights(Q, kv_pool, page_table, seqlens, m, l, weights, scale=None, causal=True):
@@ -487,15 +501,16 @@ def accumulate_weights(Q, kv_pool, page_table, seqlens, m, l, weights, scale=Non
         raise FlashDMLAError("Q and kv_pool differ in their last dimension")
     if scale is None:
         scale = 1.0 / math.sqrt(d_qk)
-    Q, m, l, page_table, seqlens = (t.contiguous() for t in (Q, m, l, page_table, seqlens))
+    Q, m, l, page_table, seqlens = Q.contiguous(), m.contiguous(), l.contiguous(), page_table.contiguous(), seqlens.contiguous()
     code, max_pages = _dtype_code(Q), page_table.shape[1]
-    with torch.cuda.device(Q.device):
+    ctx, stream = _launch_on(Q)
+    with ctx:
         L = _lib.lib()
         nbytes = L.fdmla_cache_accumulate_workspace_bytes(B, H, Sq, d_qk, page_size, max_pages, code)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=Q.device) if nbytes else None
-        check(L.fdmla_cache_accumulate(_ptr(Q), _ptr(kv_pool), _ptr(page_table), _ptr(seqlens), _ptr(m), _ptr(l), _ptr(weights),
-                                       _ptr(ws), nbytes, B, H, Sq, d_qk, page_size, max_pages, num_pages, float(scale),
-                                       int(bool(causal)), code, _stream(Q)), "fdmla_cache_accumulate")
+        check(L.fdmla_cache_accumulate(Q.data_ptr(), kv_pool.data_ptr(), page_table.data_ptr(), seqlens.data_ptr(), m.data_ptr(),
+                                       l.data_ptr(), weights.data_ptr(), _ptr(ws), nbytes, B, H, Sq, d_qk, page_size, max_pages,
+                                       num_pages, float(scale), int(bool(causal)), code, stream), "fdmla_cache_accumulate")
     return weights
 
 
@@ -515,14 +530,16 @@ def cache_evict(kv_pool, weights, positions, page_table, seqlens, next_position,
     num_pages, page_size, d_qk = kv_pool.shape
     max_pages, dev = page_table.shape[1], kv_pool.device
     page_table, seqlens, next_position = page_table.contiguous(), seqlens.contiguous(), next_position.contiguous()
+    code = _dtype_code(kv_pool)
     kept = torch.empty(B, keep, dtype=torch.int32, device=dev)
     new_seqlens = torch.empty(B, dtype=torch.int32, device=dev)
-    with torch.cuda.device(dev):
+    ctx, stream = _launch_on(kv_pool)
+    with ctx:
         L = _lib.lib()
         nbytes = L.fdmla_cache_evict_workspace_bytes(B, keep, page_size, max_pages)
         ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
-        check(L.fdmla_cache_evict(_ptr(kv_pool), _ptr(weights), _ptr(positions), _ptr(page_table), _ptr(seqlens),
-                                  _ptr(next_position), _ptr(kept), _ptr(new_seqlens), _ptr(ws), ws.numel(), B, keep, recent,
-                                  d_qk, page_size, max_pages, num_pages, _dtype_code(kv_pool), _stream(kv_pool)),
-              "fdmla_cache_evict")
+        check(L.fdmla_cache_evict(kv_pool.data_ptr(), weights.data_ptr(), positions.data_ptr(), page_table.data_ptr(),
+                                  seqlens.data_ptr(), next_position.data_ptr(), kept.data_ptr(), new_seqlens.data_ptr(),
+                                  ws.data_ptr(), max(nbytes, 16), B, keep, recent, d_qk, page_size, max_pages, num_pages, code,
+                                  stream), "fdmla_cache_evict")
     return kept, new_seqlens
