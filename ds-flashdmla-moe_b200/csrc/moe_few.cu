@@ -60,9 +60,16 @@ __global__ void __launch_bounds__(GATE_THREADS, TOK == 1 ? 1 : 2) gate_kernel(co
             wv[i] = (r < rows && e < E) ? __ldg(Wg + (size_t)(r0 + r) * E + e) : 0.f;
         }
         __syncthreads();
-        for (int i = threadIdx.x; i < ROWS * TOK; i += GATE_THREADS) {
-            const int r = i % ROWS, j = i / ROWS;
-            s_x[r][j] = (r < rows && t0 + j < n_tok) ? (double)to_f32(x[(size_t)(t0 + j) * d + r0 + r]) : 0.0;
+        {   // a warp stages 1 / (16 / TOK) of a token's rows; all loads in flight
+            const int j = warp % TOK, part0 = (warp / TOK) * 32 + lane;
+            float v[ROWS * TOK / GATE_THREADS];
+#pragma unroll
+            for (int i = 0; i < ROWS * TOK / GATE_THREADS; ++i) {
+                const int r = part0 + i * (GATE_THREADS / TOK);
+                v[i] = (r < rows && t0 + j < n_tok) ? to_f32(x[(size_t)(t0 + j) * d + r0 + r]) : 0.f;
+            }
+#pragma unroll
+            for (int i = 0; i < ROWS * TOK / GATE_THREADS; ++i) s_x[part0 + i * (GATE_THREADS / TOK)][j] = (double)v[i];
         }
         __syncthreads();
 #pragma unroll
@@ -107,7 +114,7 @@ static int launch_gate(const void *x, const float *Wg, double *part, unsigned *c
 // slices of d: one round of blocks, at least 64 rows each
 static int gate_slices(int n_tok, int d, int E) {
     const int blocks = ((E + 31) / 32) * ((n_tok + GATE_TOK - 1) / GATE_TOK);
-    int s = n_tok == 1 ? kNumSMs / blocks : (2 * kNumSMs + blocks - 1) / blocks;
+    int s = (n_tok == 1 ? 1 : 2) * kNumSMs / blocks;
     if (s > MAX_SLICES) s = MAX_SLICES;
     if (s > d / 64) s = d / 64;
     return s < 1 ? 1 : s;
@@ -125,8 +132,8 @@ __device__ __forceinline__ double key_logit(unsigned long long key) {
 // The k winners of one token by one warp; key [E] (shared memory) is overwritten.  `nan`: some logit of the token is NaN, and
 // so are its weights then, as those of a softmax over the logits would be.  Every lane keeps the best of its experts, a round
 // is three warp reductions (high half, low half, index) and a new scan by the lane that lost its best.
-__device__ __forceinline__ void topk_warp(unsigned long long *key, int E, int k, bool nan, int32_t *__restrict__ idx,
-                                          float *__restrict__ w, int lane) {
+__device__ __forceinline__ void topk_warp(unsigned long long *key, int E, int k, bool nan, int32_t *idx, float *w,
+                                          int lane) {
     unsigned long long best = 0;
     int at = 0x7fffffff;
     auto scan = [&]() {

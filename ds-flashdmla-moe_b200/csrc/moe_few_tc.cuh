@@ -46,6 +46,8 @@ template <int NP> struct TcShared {                   // behind the ring
     uint64_t bars[2 * 6 + 4 + QUEUE];
     uint32_t tmem, queue[QUEUE], ahead[6], scan[16];
     int n_routed, n_groups, last, dead;
+    int32_t idx[32];                                  // a single token's choices and their weights
+    float w[32];
     uint16_t expert[EXPERTS];                         // routed experts, ascending
     uint16_t first[EXPERTS + 1];                      // their first rows of h
     uint16_t group[EXPERTS + 2 + ROWS / GROUP];       // routed expert (or n_routed: the shared one) | second group << 15
@@ -126,18 +128,19 @@ layer_kernel(const TcProblem p, const __grid_constant__ CUtensorMap tmX, const _
     if (warp == 1) { tmem_alloc(smem_u32(&sh.tmem), C::COLS); tmem_relinquish(); }
     wait_for_primary();                                // the gate kernel's logits and zeroed counters
 
-    // ---- top-k: one token per CTA, in shared memory that the ring uses later ---------------------------------------------------
+    // ---- top-k: a token per CTA, in shared memory that the ring uses later ---------------------------------------------------
     unsigned long long *s_key = reinterpret_cast<unsigned long long *>(ring);
-    for (int t = blockIdx.x; t < p.n_tok; t += gridDim.x) {
+    const bool single = p.n_tok == 1;                  // one token: every CTA for itself, no barrier
+    for (int t = single ? 0 : blockIdx.x; t < p.n_tok; t += gridDim.x) {
         const bool nan = __syncthreads_or(token_keys(p.part + (size_t)t * p.E, p.slices, (size_t)p.n_tok * p.E, p.E, s_key));
-        if (warp == 0) topk_warp(s_key, p.E, p.k, nan, p.idx + (size_t)t * p.k, p.w + (size_t)t * p.k, lane);
+        if (warp == 0) topk_warp(s_key, p.E, p.k, nan, single ? sh.idx : p.idx + (size_t)t * p.k, single ? sh.w : p.w + (size_t)t * p.k, lane);
         __syncthreads();
     }
     // which tokens chose an expert: a 128-bit mask each
     uint32_t(*s_mask)[4] = reinterpret_cast<uint32_t(*)[4]>(ring + 16384);
     uint16_t *s_first = reinterpret_cast<uint16_t *>(ring + 16384 + MAX_E * 16), *s_idx = s_first + MAX_E;
     for (int i = tid; i < p.E * 4; i += TC_THREADS) (&s_mask[0][0])[i] = 0u;
-    if (tid == 0 && !sh.dead) {
+    if (tid == 0 && !sh.dead && !single) {
         red_release_gpu(p.bars);
         if (!grid_wait(p.bars, gridDim.x)) { sh.dead = 1; atomicCAS(&g_few_error, 0, ERR_GRID); }
     }
@@ -149,7 +152,7 @@ layer_kernel(const TcProblem p, const __grid_constant__ CUtensorMap tmX, const _
     // ---- routed experts in ascending order, their rows of h in token order (the same in every CTA) -------------------------------
     if (!dead)
         for (int i = tid; i < choices; i += TC_THREADS) {
-            const int e = __ldcg(p.idx + i), t = i / p.k;
+            const int e = single ? sh.idx[i] : __ldcg(p.idx + i), t = i / p.k;
             s_idx[i] = (uint16_t)e;
             atomicOr(&s_mask[e][t >> 5], 1u << (t & 31));
         }
@@ -483,19 +486,47 @@ layer_kernel(const TcProblem p, const __grid_constant__ CUtensorMap tmX, const _
                 // tiles cut along their reduction: all CTAs sum the pieces, in order, and write h
                 if (L == 0 && !dead && !grid_wait(p.bars + 1, gridDim.x)) atomicCAS(&g_few_error, 0, ERR_GRID);
                 named_bar_sync(1, 128);
-                const unsigned elems = dead ? 0u : (unsigned)p.rows * (unsigned)p.f;
-                for (unsigned u = blockIdx.x * 128 + L; u < elems; u += gridDim.x * 128) {
-                    const unsigned r = u / p.f, c = u - r * p.f;
-                    const float *o = p.pieces + (size_t)r * 2 * ld1 + c;
-                    float v1[16], v3[16], x1 = 0.f, x3 = 0.f;
+                // one column a thread and all pieces in flight for few tokens (latency), four columns beyond (fewer rounds); not both
+                // in one kernel, whose first launch after other work waits for its instructions
+                const unsigned elems = dead ? 0u : (unsigned)p.rows * (unsigned)p.f, threads = gridDim.x * 128;
+                if constexpr (NP == 16) {
+                    for (unsigned u = blockIdx.x * 128 + L; u < elems; u += threads) {
+                        const unsigned r = u / p.f, c = u - r * p.f;
+                        const float *o = p.pieces + (size_t)r * 2 * ld1 + c;
+                        float v1[16], v3[16], x1 = 0.f, x3 = 0.f;
 #pragma unroll
-                    for (unsigned z = 0; z < 16; ++z) {
-                        v1[z] = z < it1.split ? __ldcg(o + z * slab1) : 0.f;
-                        v3[z] = z < it1.split ? __ldcg(o + z * slab1 + ld1) : 0.f;
+                        for (unsigned z = 0; z < 16; ++z) {
+                            v1[z] = z < it1.split ? __ldcg(o + z * slab1) : 0.f;
+                            v3[z] = z < it1.split ? __ldcg(o + z * slab1 + ld1) : 0.f;
+                        }
+#pragma unroll
+                        for (unsigned z = 0; z < 16; ++z) { x1 += v1[z]; x3 += v3[z]; }
+                        p.h[u] = __float2bfloat16_rn(silu(x1) * x3);
                     }
+                } else {
+                    for (unsigned u = (blockIdx.x * 128 + L) * 4; u < elems; u += threads * 4) {
+                        const unsigned r = u / p.f, c = u - r * p.f;
+                        const float *o = p.pieces + (size_t)r * 2 * ld1 + c;
+                        float x1[4] = {}, x3[4] = {};
+                        for (unsigned z0 = 0; z0 < it1.split; z0 += 8) {
+                            float4 v1[8], v3[8];
 #pragma unroll
-                    for (unsigned z = 0; z < 16; ++z) { x1 += v1[z]; x3 += v3[z]; }
-                    p.h[u] = __float2bfloat16_rn(silu(x1) * x3);
+                            for (unsigned z = 0; z < 8; ++z) {
+                                const bool in = z0 + z < it1.split;
+                                const float *q = o + (z0 + z) * slab1;
+                                v1[z] = in ? __ldcg(reinterpret_cast<const float4 *>(q)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                                v3[z] = in ? __ldcg(reinterpret_cast<const float4 *>(q + ld1)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                            }
+#pragma unroll
+                            for (unsigned z = 0; z < 8; ++z) {
+                                x1[0] += v1[z].x; x1[1] += v1[z].y; x1[2] += v1[z].z; x1[3] += v1[z].w;
+                                x3[0] += v3[z].x; x3[1] += v3[z].y; x3[2] += v3[z].z; x3[3] += v3[z].w;
+                            }
+                        }
+                        const __nv_bfloat162 lo = __floats2bfloat162_rn(silu(x1[0]) * x3[0], silu(x1[1]) * x3[1]),
+                                             hi = __floats2bfloat162_rn(silu(x1[2]) * x3[2], silu(x1[3]) * x3[3]);
+                        *reinterpret_cast<uint2 *>(p.h + u) = make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
+                    }
                 }
                 arrive(3);
             }
@@ -512,25 +543,25 @@ layer_kernel(const TcProblem p, const __grid_constant__ CUtensorMap tmX, const _
     const size_t slab = (size_t)p.rows * p.d;
     const int n = p.k + p.shared;
     const long long threads = (long long)gridDim.x * TC_THREADS, me = (long long)blockIdx.x * TC_THREADS + tid;
-    // V columns a thread, J choices' pieces (four each) in flight
+    // V columns a thread (one for few tokens, four beyond), Z pieces each of J choices in flight
     auto weighted_sum = [&](auto v_, auto j_) {
-        constexpr int V = decltype(v_)::value, J = decltype(j_)::value;
+        constexpr int V = decltype(v_)::value, J = decltype(j_)::value, Z = 4;
         const int per_row = p.d / V;
         for (long long u = me; u < (long long)p.n_tok * per_row; u += threads) {
             const int t = (int)(u / per_row), c = (int)(u - (long long)t * per_row) * V;
             float sum[V] = {};
             for (int j0 = 0; j0 < n; j0 += J) {
                 float y[J][V] = {}, g[J];
-                for (unsigned z0 = 0; z0 < it2.split; z0 += 4) {
-                    float v[J][4][V];
+                for (unsigned z0 = 0; z0 < it2.split; z0 += Z) {
+                    float v[J][Z][V];
 #pragma unroll
                     for (int j = 0; j < J; ++j) {
                         const bool in = j0 + j < n, own = j0 + j >= p.k;
                         const size_t row = !in ? 0 : own ? choices + t : sh.row[t * p.k + j0 + j];
                         const float *src = p.pieces + row * p.d + c;
-                        if (z0 == 0) g[j] = !in || own ? 1.f : __ldcg(p.w + (size_t)t * p.k + j0 + j);
+                        if (z0 == 0) g[j] = !in || own ? 1.f : single ? sh.w[j0 + j] : __ldcg(p.w + (size_t)t * p.k + j0 + j);
 #pragma unroll
-                        for (unsigned z = 0; z < 4; ++z) {
+                        for (unsigned z = 0; z < Z; ++z) {
                             const bool ld = in && z0 + z < it2.split;
                             if constexpr (V == 4) {
                                 const float4 q = ld ? __ldcg(reinterpret_cast<const float4 *>(src + (z0 + z) * slab)) : make_float4(0.f, 0.f, 0.f, 0.f);
@@ -541,7 +572,7 @@ layer_kernel(const TcProblem p, const __grid_constant__ CUtensorMap tmX, const _
 #pragma unroll
                     for (int j = 0; j < J; ++j)
 #pragma unroll
-                        for (int z = 0; z < 4; ++z)
+                        for (int z = 0; z < Z; ++z)
 #pragma unroll
                             for (int i = 0; i < V; ++i) y[j][i] += v[j][z][i];
                 }
@@ -558,8 +589,7 @@ layer_kernel(const TcProblem p, const __grid_constant__ CUtensorMap tmX, const _
             } else *o = __float2bfloat16_rn(sum[0]);
         }
     };
-    // one column a thread while that is at most one round (latency), four beyond
-    if ((long long)p.n_tok * p.d <= threads) weighted_sum(std::integral_constant<int, 1>{}, std::integral_constant<int, 9>{});
+    if constexpr (NP == 16) weighted_sum(std::integral_constant<int, 1>{}, std::integral_constant<int, 9>{});
     else weighted_sum(std::integral_constant<int, 4>{}, std::integral_constant<int, 4>{});
 }
 
