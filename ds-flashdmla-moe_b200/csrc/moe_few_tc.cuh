@@ -218,6 +218,8 @@ layer_kernel(const TcProblem p, const __grid_constant__ CUtensorMap tmX, const _
         row0 = a < routed ? (int)sh.first[a] : choices;
         return (a < routed ? (int)sh.first[a + 1] : choices + p.n_tok) - row0;
     };
+    // stage 1 begins with the shared expert: with several tokens its tiles take longest
+    auto expert_of = [&](unsigned i) { return !p.shared ? i : (i == 0 ? routed : i - 1); };
     auto group_of = [&](unsigned g, unsigned &a, int &row0) {
         a = sh.group[g] & 0x7fff;
         const int skip = sh.group[g] >> 15 ? GROUP : 0, n = rows_of(a, row0) - skip;
@@ -244,7 +246,7 @@ layer_kernel(const TcProblem p, const __grid_constant__ CUtensorMap tmX, const _
         for (unsigned item = blockIdx.x; ok && item < it1.total; item = __shfl_sync(0xffffffffu, ans, 0)) {
             ans = ask(1, gridDim.x);
             announce(item);
-            const unsigned i = item % p.ft, q = item / p.ft, a = q / it1.split, ks = q - a * it1.split;
+            const unsigned i = item % p.ft, q = item / p.ft, ks = q % it1.split, a = expert_of(q / it1.split);
             const bool own = a >= routed;
             const CUtensorMap *m1 = own ? &tmS1 : &tmW1, *m3 = own ? &tmS3 : &tmW3;
             const int row0 = own ? 0 : (int)sh.expert[a] * p.d;
@@ -448,7 +450,7 @@ layer_kernel(const TcProblem p, const __grid_constant__ CUtensorMap tmX, const _
                     mbar_arrive(ACC_EMPTY(acc));
                     continue;
                 }
-                const unsigned i1 = item % p.ft, q = item / p.ft, a = q / it1.split, ks = q - a * it1.split;
+                const unsigned i1 = item % p.ft, q = item / p.ft, ks = q % it1.split, a = expert_of(q / it1.split);
                 int row0;
                 const int n = rows_of(a, row0), col = (int)i1 * 128 + L;
                 float *piece = p.pieces + (size_t)row0 * 2 * ld1 + col;          // of split 0
