@@ -435,7 +435,7 @@ static bool pages_ok(int B, int page_size, int max_pages, int num_pages) {
 
 extern "C" size_t fdmla_cache_accumulate_workspace_bytes(int B, int H, int Sq, int d_qk, int page_size, int max_pages, int dtype) {
     if (B <= 0 || H <= 0 || Sq <= 0 || d_qk <= 0 || page_size <= 0 || max_pages <= 0) return 0;
-    if (!cw::accumulate_tc_supported(B, (long long)H * Sq, d_qk, page_size, 1, dtype)) return 0;
+    if (!cw::accumulate_tc_supported(B, (long long)H * Sq, d_qk, page_size, max_pages, 1, dtype)) return 0;
     const long long cap = (long long)page_size * max_pages;
     const int splits = cw::row_splits(B, (long long)H * Sq, cap);
     return splits > 1 ? (size_t)splits * B * cap * sizeof(float) : 0;
@@ -458,7 +458,7 @@ extern "C" int fdmla_cache_accumulate(const void *Q, const void *kv_pool, const 
     p.B = B; p.R = H * Sq; p.Sq = Sq; p.d = d_qk; p.causal = causal ? 1 : 0;
     p.scale_log2 = scale * 1.4426950408889634f;
     cudaStream_t s = (cudaStream_t)stream;
-    const bool tc = cw::accumulate_tc_supported(B, p.R, d_qk, page_size, num_pages, dtype) &&
+    const bool tc = cw::accumulate_tc_supported(B, p.R, d_qk, page_size, max_pages, num_pages, dtype) &&
                     ((reinterpret_cast<uintptr_t>(Q) | reinterpret_cast<uintptr_t>(kv_pool)) & 15) == 0;
     if (fdmla_get_backend() == FDMLA_BACKEND_TENSOR && !tc) return FDMLA_ERR_UNSUPPORTED;
     if (tc && tensor_kernels_allowed()) {
@@ -466,7 +466,8 @@ extern "C" int fdmla_cache_accumulate(const void *Q, const void *kv_pool, const 
         return cw::run_accumulate_tc(p, workspace, s);
     }
     note_kernel("portable");
-    const long long smem = 32LL * (d_qk + 1) * 4;
+    // the keys' rows, then the warps' sums in the same place (more than the rows for d < 7)
+    const long long rows = 32LL * (d_qk + 1) * 4, sums = cw::ACC_WARPS * 32 * 4, smem = rows > sums ? rows : sums;
     if (smem > kMaxSmemPerBlock) return FDMLA_ERR_UNSUPPORTED;
     const dim3 grid((unsigned)(((long long)max_pages * page_size + 31) / 32), B);
     const void *fn = dtype == FDMLA_F32 ? (const void *)cw::accumulate_simt_kernel<float> : (const void *)cw::accumulate_simt_kernel<__nv_bfloat16>;
@@ -502,8 +503,8 @@ extern "C" int fdmla_cache_evict(void *kv_pool, float *weights, int32_t *positio
     if (dtype != FDMLA_F32 && dtype != FDMLA_BF16) return FDMLA_ERR_INVALID;
     if (B == 0) return FDMLA_OK;
     if (!kv_pool || !weights || !positions || !page_table || !seqlens || !next_position || !kept || !new_seqlens) return FDMLA_ERR_INVALID;
-    if (!pages_ok(B, page_size, max_pages, num_pages)) return FDMLA_ERR_UNSUPPORTED;
-    if (max_pages > 0 && (!workspace || workspace_bytes < fdmla_cache_evict_workspace_bytes(B, keep, page_size, max_pages))) return FDMLA_ERR_WORKSPACE;
+    if (!pages_ok(B, page_size, max_pages, num_pages) || keep > (1 << 30)) return FDMLA_ERR_UNSUPPORTED;
+    if (max_pages > 0 && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 3) || workspace_bytes < fdmla_cache_evict_workspace_bytes(B, keep, page_size, max_pages))) return FDMLA_ERR_WORKSPACE;
     cudaStream_t s = (cudaStream_t)stream;
     const int cap = page_size * max_pages;
     // CTAs per sequence: enough for every SM as long as a CTA keeps a few thousand rows, and room for the keys of the longest
@@ -555,7 +556,7 @@ extern "C" int fdmla_cache_evict(void *kv_pool, float *weights, int32_t *positio
     cudaError_t e;
     if (row_bytes % 16 == 0 && (reinterpret_cast<uintptr_t>(kv_pool) & 15) == 0)
         e = cudaLaunchKernelEx(&mv, cw::move_kernel<uint4>, pool, weights, positions, k, p.pg, B, keep, row_bytes, span);
-    else if (row_bytes % 4 == 0)
+    else if (row_bytes % 4 == 0 && (reinterpret_cast<uintptr_t>(kv_pool) & 3) == 0)
         e = cudaLaunchKernelEx(&mv, cw::move_kernel<unsigned int>, pool, weights, positions, k, p.pg, B, keep, row_bytes, span);
     else
         e = cudaLaunchKernelEx(&mv, cw::move_kernel<unsigned short>, pool, weights, positions, k, p.pg, B, keep, row_bytes, span);

@@ -430,7 +430,8 @@ __global__ void __launch_bounds__(256) add_partials_kernel(const float *__restri
     if (row >= 0) atomicAdd(weights + row, g);
 }
 
-static bool accumulate_tc_supported(int B, long long R, int d, int page_size, int num_pages, int dtype) {
+static bool accumulate_tc_supported(int B, long long R, int d, int page_size, int max_pages, int num_pages, int dtype) {
+    if (((long long)page_size * max_pages / KEYS + 1) * B > 2147483647LL) return false;              // tiles are counted in 32 bits
     return dtype == FDMLA_BF16 && d % 64 == 0 && d <= 64 * MAX_CHUNKS && page_size % 64 == 0 && num_pages > 0 &&
            (long long)B * R + QROWS <= 2147483647LL;
 }

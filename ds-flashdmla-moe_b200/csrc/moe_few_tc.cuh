@@ -630,7 +630,7 @@ static TcLayout tc_layout(int n_tok, int d, int f, int E, int k, int shared) {
 
 static bool tc_supported(int d, int f, int E, int dtype) {
     return dtype == FDMLA_BF16 && d % 64 == 0 && f % 64 == 0 && (long long)E * d < (1LL << 31) && (long long)E * f < (1LL << 31) &&
-           f <= 65535 * 128 && (long long)(E + 1) * ((f + 127) / 128) * 16 < (1LL << 31) && (long long)(E + 66) * ((d + 127) / 128) * 16 < (1LL << 31);
+           f <= (1 << 18) && (long long)(E + 1) * ((f + 127) / 128) * 16 < (1LL << 31) && (long long)(E + 66) * ((d + 127) / 128) * 16 < (1LL << 31);
 }
 static bool tc_aligned(const Args &a) {
     return ((reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.W1) | reinterpret_cast<uintptr_t>(a.W3) |

@@ -100,8 +100,8 @@ class PagedLatentCache:
 
     def reserve(self, slots: Sequence[int], n_tokens: int) -> torch.Tensor:
         """Make room for n_tokens more rows in every listed sequence (allocating pages as needed),
-        advance the lengths and return the positions the new rows start at, [len(slots)] int32.
-        Nothing is changed if any sequence cannot be extended."""
+        advance the lengths and return the rows the new ones start at, [len(slots)] int32 (they get weight 0
+        and their positions in a cache that tracks weights).  Nothing is changed if any sequence cannot be extended."""
         if n_tokens < 0:
             raise FlashDMLAError("n_tokens must be >= 0")
         if len(set(slots)) != len(slots):
@@ -117,6 +117,7 @@ class PagedLatentCache:
         if sum(need) > len(self._free_pages):
             raise FlashDMLAError(f"out of cache pages: need {sum(need)}, {len(self._free_pages)} free")
         start = torch.empty(len(slots), dtype=torch.int32)
+        first = torch.tensor([int(self.h_next[s]) for s in slots], dtype=torch.int32)
         for i, (s, k) in enumerate(zip(slots, need)):
             for _ in range(k):
                 pg = self._free_pages.pop()
@@ -126,6 +127,9 @@ class PagedLatentCache:
             self.h_len[s] += n_tokens
             self.h_next[s] += n_tokens
         self._sync_rows(slots)
+        if self.on_gpu and self.track_weights and n_tokens > 0 and len(slots) > 0:
+            table, _ = self.tables(slots)
+            ops.cache_stamp(self.weights, self.positions, table, start.to(self.device), first.to(self.device), n_tokens)
         return start
 
     # ------------------------------------------------------------------ device side
@@ -138,13 +142,9 @@ class PagedLatentCache:
             raise FlashDMLAError("rows must be [len(slots), n_tokens, d_qk]")
         if not self.on_gpu:
             raise FlashDMLAError("append needs a CUDA cache (there is no CPU fallback)")
-        first = torch.tensor([self.position(s) for s in slots], dtype=torch.int32)
         start = self.reserve(slots, rows.shape[1])
         idx = torch.tensor(list(slots), dtype=torch.long, device=self.device)
-        table, d_start = self.d_table.index_select(0, idx), start.to(self.device)
-        ops.cache_append(rows, self.pool, table, d_start)
-        if self.track_weights:
-            ops.cache_stamp(self.weights, self.positions, table, d_start, first.to(self.device), rows.shape[1])
+        ops.cache_append(rows, self.pool, self.d_table.index_select(0, idx), start.to(self.device))
         return start
 
     def tables(self, slots: Sequence[int]):

@@ -109,8 +109,8 @@ def moe_few(x: torch.Tensor, Wg: torch.Tensor, W1: torch.Tensor, W3: torch.Tenso
     W2 [E,f,d], shared = (S1 [d,f], S3 [d,f], S2 [f,d]) or None -> [T,d] in x's dtype.
 
     The k experts with the largest logit win (ties: the lower expert), their outputs are weighted with the softmax over the
-    winners' logits; there is no capacity and nothing is dropped.  Every chosen expert's weights are read once.  Weights have
-    to be finite.  out: a contiguous tensor to write into."""
+    winners' logits; there is no capacity and nothing is dropped.  Every chosen expert's weights are read once.
+    Forward only.  out: a contiguous tensor to write into."""
     _need_cuda(x, Wg, W1, W3, W2, *(shared or ()))
     if x.dim() != 2 or W1.dim() != 3:
         raise FlashDMLAError("expected x [T,d], Wg [d,E], W1, W3 [E,d,f], W2 [E,f,d]")
@@ -123,6 +123,8 @@ def moe_few(x: torch.Tensor, Wg: torch.Tensor, W1: torch.Tensor, W3: torch.Tenso
         raise FlashDMLAError("x and the expert weights must share one dtype")
     s1 = s3 = s2 = None
     if shared is not None:
+        if len(shared) != 3:
+            raise FlashDMLAError("the shared expert must be (S1 [d,f], S3 [d,f], S2 [f,d])")
         S1, S3, S2 = shared
         if S1.shape != (d, f) or S3.shape != (d, f) or S2.shape != (f, d):
             raise FlashDMLAError("the shared expert must be (S1 [d,f], S3 [d,f], S2 [f,d])")

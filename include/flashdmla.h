@@ -70,8 +70,9 @@ int fdmla_set_single_cta(int on);
 const char *fdmla_last_kernel(void);
 
 /* Device-side error flag of the tensor-core kernels on the current device:
- * 0 = none; 1..3, 11..17, 21..23 and 31 = a bounded wait inside a kernel gave up (which
- * kernel, role and wait; 31: a peer of fdmla_exchange_merge did not arrive); 4 = a page id outside [0, num_pages) was read from a page
+ * 0 = none; 1..3, 11..17, 21..23, 31, 41..44 and 51..53 = a bounded wait inside a kernel gave up (which
+ * kernel, role and wait; 31: a peer of fdmla_exchange_merge did not arrive; 41..44: fdmla_moe_few,
+ * 51..53: fdmla_cache_accumulate, whose later launches leave their outputs as they were); 4 = a page id outside [0, num_pages) was read from a page
  * table, or a sequence length outside [0, max_pages * page_size] was clamped.
  * Synchronises the device; reset != 0 clears the flag.  Returns -1 if the flag
  * cannot be read.
@@ -446,7 +447,7 @@ int fdmla_cache_accumulate(const void *Q, const void *kv_pool,
  *   Rows from `keep` on keep their contents.
  *   kept [B, keep] int32 (out): the row that row j held before the call, -1 for j past the new end.
  *   new_seqlens [B] int32 (out): min(seqlens[b], keep); may be the array seqlens itself.
- *   0 <= recent <= keep, keep >= 1.  The sequences of one call must not share pages.  page_size * max_pages at most
+ *   0 <= recent <= keep, 1 <= keep <= 2^30.  The sequences of one call must not share pages.  page_size * max_pages at most
  *   785 000 rows (FDMLA_ERR_UNSUPPORTED beyond).  A row on a bad page counts as the lightest and is not copied (code 4).
  *   workspace: fdmla_cache_evict_workspace_bytes() bytes of device scratch.
  */
@@ -532,9 +533,8 @@ int fdmla_moe_combine(const void *y, const int32_t *pos, const float *w,
  *   x [T, d], Wg [d, E] fp32, W1, W3 [E, d, f], W2 [E, f, d], shared expert S1, S3 [d, f], S2 [f, d] (all three NULL: none),
  *   out [T, d]; x, W*, S*, out in `dtype`.  There is no capacity: nothing is dropped.
  *   The logits are summed in 64 bits.  bf16 with d and f multiples of 64 runs on the tensor cores: the intermediate
- *   activation, gate weight included, is rounded to bf16 once, sums are fp32, out is rounded once.  An expert that any token
- *   of the call chooses multiplies all of the call's tokens with zeros for the others: weights must be finite there.
- *   Everything else runs on CUDA cores with an fp32 intermediate.
+ *   activation, gate weight included, is rounded to bf16 once, sums are fp32, out is rounded once.  Everything else runs on
+ *   CUDA cores with an fp32 intermediate.
  *   k <= min(E, 32), E <= 2048; workspace: fdmla_moe_few_workspace_bytes() bytes of device scratch, 256-byte aligned.
  */
 size_t fdmla_moe_few_workspace_bytes(int T, int d, int f, int E, int k,

@@ -485,3 +485,120 @@ def test_block_step_with_bounded_cache_and_few_token_moe(cuda):
         c.evict(slots, keep=90, recent=10)
         assert all(c.length(s) == 90 and c.position(s) == 101 + step for s in slots)
         assert all(101 + step - 1 in c.row_state(s)[1].tolist() for s in slots)     # the newest row is still there
+
+
+# ------------------------------------------------------------------------------------------ pointers, streams, far pages
+@pytest.mark.gpu
+@pytest.mark.parametrize("d,shift", [(6, 1), (6, 2), (64, 1), (64, 2), (64, 8)])
+def test_pools_that_start_at_odd_addresses(cuda, d, shift):
+    """A pool (and Q) that is a view `shift` elements into a larger buffer: wide copies and bulk copies may not be used."""
+    import flashdmla as F
+    lens, keep = [150, 70, 10], 60
+    case = evict_case(lens, keep, 9, 64, d, torch.bfloat16, "random", 21)
+    pool, weights, positions, table, phys, nxt = case
+
+    def view(t):
+        buf = torch.zeros(t.numel() + 32, dtype=t.dtype, device=cuda)
+        v = buf[shift:shift + t.numel()].view(t.shape)
+        v.copy_(t)
+        return v
+    dlens = torch.tensor(lens, dtype=torch.int32, device=cuda)
+    # accumulate first, on clean rows
+    g = torch.Generator().manual_seed(2)
+    Q = torch.randn(len(lens), 4, 1, d, generator=g).to(torch.bfloat16)
+    scale = 1.0 / math.sqrt(d)
+    st = [stats(Q[b], pool.view(-1, d)[r], scale) for b, r in enumerate(phys)]
+    m, l = torch.stack([s[0] for s in st]), torch.stack([s[1] for s in st])
+    w = weights.to(cuda)
+    F.accumulate_weights(view(Q), view(pool), table.to(cuda), dlens, m.to(cuda), l.to(cuda), w, scale)
+    check_accumulated(w.cpu(), (pool, table, phys, Q, weights, scale, m, l), True)
+    dp, dw, dpos = view(pool), weights.to(cuda), positions.to(cuda)
+    kept, new = F.cache_evict(dp, dw, dpos, table.to(cuda), dlens, torch.tensor(nxt, dtype=torch.int32, device=cuda), keep, 9)
+    check_evicted((dp.cpu(), dw.cpu(), dpos.cpu(), kept.cpu(), new.cpu()), case, lens, keep, 9)
+    assert F.device_error_flag() == 0
+
+
+@pytest.mark.gpu
+def test_pages_behind_two_to_the_31_elements(cuda):
+    """Pages whose first element lies beyond 2^31 elements (4 GB) of the pool."""
+    import flashdmla as F
+    g = torch.Generator().manual_seed(6)
+    lens, d, H, keep = [200, 321], 576, 16, 130
+    small, table, phys = paged(lens, 64, d, torch.bfloat16, g)
+    N = 60000
+    far = torch.randperm(1000, generator=g)[: small.shape[0]].sort().values + (N - 1000)
+    pool = torch.empty(N, 64, d, dtype=torch.bfloat16, device=cuda)
+    pool[far.to(cuda)] = small.to(cuda)
+    ftable = far[table.long()].to(torch.int32)
+    Q = torch.randn(2, H, 1, d, generator=g).to(torch.bfloat16)
+    scale = 1 / math.sqrt(d)
+    st = [stats(Q[b], small.view(-1, d)[r], scale) for b, r in enumerate(phys)]
+    m, l = torch.stack([s[0] for s in st]), torch.stack([s[1] for s in st])
+    weights = torch.randn(small.shape[:2], generator=g).exp()
+    big_w = torch.zeros(N, 64, device=cuda)
+    big_w[far.to(cuda)] = weights.to(cuda)
+    dlens = torch.tensor(lens, dtype=torch.int32, device=cuda)
+    F.accumulate_weights(Q.to(cuda), pool, ftable.to(cuda), dlens, m.to(cuda), l.to(cuda), big_w, scale)
+    check_accumulated(big_w[far.to(cuda)].cpu(), (small, table, phys, Q, weights, scale, m, l), True)
+    positions = torch.zeros(small.shape[:2], dtype=torch.int32)
+    case = (small, weights, positions, table, phys, [1000, 1000])
+    big_w[far.to(cuda)] = weights.to(cuda)
+    big_p = torch.zeros(N, 64, dtype=torch.int32, device=cuda)
+    kept, new = F.cache_evict(pool, big_w, big_p, ftable.to(cuda), dlens, torch.full((2,), 1000, dtype=torch.int32, device=cuda), keep)
+    check_evicted((pool[far.to(cuda)].cpu(), big_w[far.to(cuda)].cpu(), big_p[far.to(cuda)].cpu(), kept.cpu(), new.cpu()), case, lens, keep, 0)
+    assert F.device_error_flag() == 0
+
+
+@pytest.mark.gpu
+def test_accumulate_shared_pages_streams_and_graph(cuda):
+    """Two sequences on the same pages add up; calls on two streams do not disturb each other; a captured call replays."""
+    import flashdmla as F
+    lens, H, d = [300, 300], 32, 576
+    pool, table, phys, Q, weights, scale, m, l = acc_inputs(lens, H, 1, d, 64, torch.bfloat16, True)
+    table[1] = table[0]
+    st = [stats(Q[b], pool.view(-1, d)[phys[0]], scale) for b in range(2)]
+    m, l = torch.stack([s[0] for s in st]), torch.stack([s[1] for s in st])
+    want, tol = weights.double().clone().view(-1), torch.zeros(weights.numel(), dtype=torch.float64)
+    for b in range(2):
+        w, e = accumulate_oracle(Q[b], pool.view(-1, d)[phys[0]], m[b], l[b], scale)
+        want[phys[0]] += w
+        tol[phys[0]] += e
+    tol += 2 * 2.0 ** -23 * want.abs()
+    args = [t.to(cuda) for t in (Q, pool, table, torch.tensor(lens, dtype=torch.int32), m, l)]
+    bufs = [weights.to(cuda) for _ in range(4)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(device=cuda) for _ in range(2)]
+    for i, b in enumerate(bufs):
+        with torch.cuda.stream(streams[i % 2]):
+            F.accumulate_weights(*args, b, scale)
+    torch.cuda.synchronize()
+    for b in bufs:
+        assert ((b.cpu().double().view(-1) - want).abs() <= tol).all()
+    w = weights.to(cuda)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        F.accumulate_weights(*args, w, scale)
+    for _ in range(2):
+        w.copy_(weights)
+        g.replay()
+        torch.cuda.synchronize()
+        assert ((w.cpu().double().view(-1) - want).abs() <= tol).all()
+
+
+@pytest.mark.gpu
+def test_reserved_rows_start_without_weight(cuda):
+    """Pages handed on to another sequence do not carry over weights or positions, however their rows are written."""
+    from flashdmla import PagedLatentCache
+    c = PagedLatentCache(num_pages=4, page_size=64, d_qk=64, max_seqs=2, max_pages_per_seq=4, device=cuda, track_weights=True)
+    a = c.new_sequence()
+    c.append([a], torch.randn(1, 200, 64, device=cuda).bfloat16())
+    c.decode(torch.randn(1, 4, 64, device=cuda).bfloat16(), [a], 64)
+    assert (c.row_state(a)[0] > 0).all() and c.row_state(a)[1].tolist() == list(range(200))
+    c.free_sequence(a)
+    b = c.new_sequence()
+    c.reserve([b], 130)
+    w, p = c.row_state(b)
+    assert (w == 0).all() and p.tolist() == list(range(130))
+    assert c.evict([b], 100).tolist() == [list(range(100))]               # all weights equal: the lower rows stay
+    c.reserve([b], 1)
+    assert c.row_state(b)[1].tolist() == list(range(100)) + [130]

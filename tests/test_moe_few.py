@@ -171,6 +171,20 @@ def test_ties_skewed_choices_and_strange_tokens(cuda, dtype):
     rest = [t for t in range(T) if t not in (7, 11)]
     assert torch.equal(out2[rest], out[rest])
     assert out2[7].isnan().any() and not out2[11].isfinite().all()
+    # infinities in an expert's weights reach the tokens that chose it, nobody else
+    Wg2 = torch.randn(d, E, generator=torch.Generator().manual_seed(3)) / math.sqrt(d)
+    out3 = F.moe_few(*[t.to(cuda) for t in (x, Wg2, *ws)], k)
+    chose = torch.topk(x.double() @ Wg2.double(), k, dim=1).indices
+    users = (chose == 1).any(1)
+    users[4] = True                                            # the token of zeros chooses experts 0, 1, 2
+    assert 0 < int(users.sum()) < T
+    ws2 = [w.clone() for w in ws]
+    for w in ws2:
+        w[1, 3, 5] = float("inf")
+    out4 = F.moe_few(*[t.to(cuda) for t in (x, Wg2, *ws2)], k)
+    assert torch.equal(out4[~users], out3[~users])
+    users[4] = False
+    assert not out4[users].isfinite().all(dim=1).any()
     assert F.device_error_flag() == 0
 
 
@@ -236,3 +250,37 @@ def test_refusals(cuda):
     call(shared=(dsh[0], dsh[1], dsh[2][:32]))
     call(out=torch.empty(4, 64, device=cuda))
     call(out=torch.empty(64, 4, dtype=torch.bfloat16, device=cuda).t())
+
+
+@pytest.mark.gpu
+def test_tensors_that_start_at_odd_addresses(cuda):
+    """Views a few elements into larger buffers: the kernels that copy in bulk step aside."""
+    import flashdmla as F
+    x, Wg, ws, sh = weights(5, 128, 64, 6, True, torch.bfloat16, 9)
+    want, err = definition(x, Wg, ws, sh, 2)
+
+    def view(t, shift):
+        buf = torch.zeros(t.numel() + 32, dtype=t.dtype, device=cuda)
+        v = buf[shift:shift + t.numel()].view(t.shape)
+        v.copy_(t)
+        return v
+    for shift in (1, 4):
+        for which in range(9):
+            ts = [view(t, shift if i == which else 0) for i, t in enumerate((x, Wg, *ws, *sh, torch.zeros_like(x)))]
+            out = F.moe_few(*ts[:5], 2, tuple(ts[5:8]), out=ts[8])
+            check(out, want, err)
+    assert F.device_error_flag() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("seed", range(6))
+def test_random_shapes(cuda, seed):
+    import random
+    import flashdmla as F
+    r = random.Random(seed)
+    T, E = r.choice([1, 2, 3, 5, 15, 16, 17, 33, 64, 65, 100, 128]), r.randint(1, 70)
+    d, f, k = 64 * r.randint(1, 12), 64 * r.randint(1, 9), r.randint(1, min(E, 9))
+    x, Wg, ws, sh = weights(T, d, f, E, r.random() < 0.5, torch.bfloat16, 100 + seed)
+    want, err = definition(x, Wg, ws, sh, k)
+    out = F.moe_few(*[t.to(cuda) for t in (x, Wg, *ws)], k, tuple(t.to(cuda) for t in sh) if sh else None)
+    check(out, want, err)
