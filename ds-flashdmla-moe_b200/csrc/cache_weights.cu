@@ -470,8 +470,8 @@ extern "C" int fdmla_cache_accumulate(const void *Q, const void *kv_pool, const 
     const long long rows = 32LL * (d_qk + 1) * 4, sums = cw::ACC_WARPS * 32 * 4, smem = rows > sums ? rows : sums;
     if (smem > kMaxSmemPerBlock) return FDMLA_ERR_UNSUPPORTED;
     const dim3 grid((unsigned)(((long long)max_pages * page_size + 31) / 32), B);
-    const void *fn = dtype == FDMLA_F32 ? (const void *)cw::accumulate_simt_kernel<float> : (const void *)cw::accumulate_simt_kernel<__nv_bfloat16>;
-    if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmemPerBlock) != cudaSuccess) { cudaGetLastError(); return FDMLA_ERR_CUDA; }
+    if (!(dtype == FDMLA_F32 ? allow_smem<cw::accumulate_simt_kernel<float>>(kMaxSmemPerBlock)
+                             : allow_smem<cw::accumulate_simt_kernel<__nv_bfloat16>>(kMaxSmemPerBlock))) return FDMLA_ERR_CUDA;
     if (dtype == FDMLA_F32) cw::accumulate_simt_kernel<float><<<grid, cw::ACC_WARPS * 32, (size_t)smem, s>>>(p);
     else cw::accumulate_simt_kernel<__nv_bfloat16><<<grid, cw::ACC_WARPS * 32, (size_t)smem, s>>>(p);
     return check_launch();
@@ -519,8 +519,8 @@ extern "C" int fdmla_cache_evict(void *kv_pool, float *weights, int32_t *positio
     p.keep = keep; p.recent = recent; p.seg = seg; p.cap = keep < cap ? keep : cap;
     p.holes = p.movers + (size_t)B * p.cap;
     const size_t smem = (size_t)seg * 4;
-    if (cudaFuncSetAttribute(cw::select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, cw::MAX_SEG * 4) != cudaSuccess ||
-        (cs > 8 && cudaFuncSetAttribute(cw::select_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)) {
+    if (!allow_smem<cw::select_kernel>(cw::MAX_SEG * 4)) return FDMLA_ERR_CUDA;
+    if (cs > 8 && cudaFuncSetAttribute(cw::select_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) {
         cudaGetLastError();
         return FDMLA_ERR_CUDA;
     }

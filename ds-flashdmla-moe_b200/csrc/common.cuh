@@ -6,6 +6,8 @@
 #include <math_constants.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/flashdmla.h"
 
 namespace fdmla {
@@ -163,6 +165,21 @@ bool tensor_kernels_allowed();
 int wgrad_num_partials(long long rows);
 int launch_wgrad(const void *X, const float *G, float *partials, void *dW, long long rows,
                  int d_in, int d_out, int dtype, cudaStream_t stream);
+
+// Dynamic shared memory of a kernel raised to `bytes`, once per kernel and device (the runtime call costs a microsecond).
+template <auto Kernel>
+inline bool allow_smem(int bytes) {
+    static std::atomic<bool> done[64];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return false;
+    if (dev >= 0 && dev < 64 && done[dev].load(std::memory_order_relaxed)) return true;
+    if (cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) {
+        cudaGetLastError();
+        return false;
+    }
+    if (dev >= 0 && dev < 64) done[dev].store(true, std::memory_order_relaxed);
+    return true;
+}
 
 inline int check_launch() {
     cudaError_t e = cudaGetLastError();

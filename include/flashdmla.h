@@ -532,9 +532,9 @@ int fdmla_moe_combine(const void *y, const int32_t *pos, const float *w,
  *   out[t] = sum_j w[t, j] (silu(x[t] W1[e_j]) * (x[t] W3[e_j])) W2[e_j]  + (silu(x[t] S1) * (x[t] S3)) S2
  *   x [T, d], Wg [d, E] fp32, W1, W3 [E, d, f], W2 [E, f, d], shared expert S1, S3 [d, f], S2 [f, d] (all three NULL: none),
  *   out [T, d]; x, W*, S*, out in `dtype`.  There is no capacity: nothing is dropped.
- *   The logits are summed in 64 bits.  bf16 with d and f multiples of 64 runs on the tensor cores: the intermediate
- *   activation, gate weight included, is rounded to bf16 once, sums are fp32, out is rounded once.  Everything else runs on
- *   CUDA cores with an fp32 intermediate.
+ *   The logits are summed in 64 bits.  bf16 with d and f multiples of 64 (f <= 2^18) runs on the tensor cores: the
+ *   intermediate activation is rounded to bf16 once, sums are fp32, out is rounded once.  Everything else runs on CUDA cores
+ *   with an fp32 intermediate.
  *   k <= min(E, 32), E <= 2048; workspace: fdmla_moe_few_workspace_bytes() bytes of device scratch, 256-byte aligned.
  */
 size_t fdmla_moe_few_workspace_bytes(int T, int d, int f, int E, int k,
