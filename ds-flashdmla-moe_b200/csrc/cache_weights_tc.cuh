@@ -8,7 +8,8 @@
 // cover the latency of HBM (four slots of one CTA alone would hold 64 KB in flight).
 //   ROWS = false  at most 256 query rows per sequence (a decode step): they stay in shared memory while the keys of the
 //                 sequence stream past; a pair takes a contiguous run of tiles, at a change of sequence the queries are
-//                 exchanged chunk by chunk as the last MMAs release them.  Bound by reading the rows once.
+//                 exchanged chunk by chunk as the last MMAs release them (all keys ahead of all queries cost 5 us a change).
+//                 Bound by reading the rows once.
 //   ROWS = true   more query rows (a prompt, a window of queries): a tile's keys stay and the query rows stream, 256 at a time (an
 //                 MMA costs about 60 cycles to issue: with 128 the issue, not the MMA, bounds), the sums staying in registers; tiles are dealt out round robin and, when there are
 //                 few, cut along the query rows into `splits` whose partial sums a second kernel adds in order.  Bound by the
@@ -51,15 +52,16 @@ struct TcProblem {
 // One step of the resident operand's life: sequence b, resident operand set `item`, and the tiles that stream past it.
 template <bool ROWS>
 struct Walker {
-    const TcProblem &p;
+    const TcProblem *q;
     int b, tile, left;                               // ROWS = false: next tile of the run, tiles left in it
     long long item, base;                            // ROWS = true: next item; items of the sequences before b
     int n, t0, count;                                // of the located piece: keys of b, first key, streaming steps
     int r_lo;                                        // ROWS = true: first row tile
     int split;
     __device__ __forceinline__ Walker(const TcProblem &p_, const TcShared &sh, int unit)
-        : p(p_), b(ROWS ? 0 : sh.b0), tile(sh.tile0), left(sh.n_tiles), item(unit), base(0), n(0), t0(0), count(0), r_lo(0), split(0) {}
+        : q(&p_), b(ROWS ? 0 : sh.b0), tile(sh.tile0), left(sh.n_tiles), item(unit), base(0), n(0), t0(0), count(0), r_lo(0), split(0) {}
     __device__ __forceinline__ bool next(int units) {
+        const TcProblem &p = *q;
         if (ROWS) {
             for (; b < p.a.B; ++b) {
                 n = p.a.pg.length(b);
@@ -91,6 +93,7 @@ struct Walker {
     }
     // does row tile r see any key of the piece
     __device__ __forceinline__ bool sees(int r) const {
+        const TcProblem &p = *q;
         if (!p.a.causal) return true;
         const int q0 = r * QROWS % p.a.Sq, q1 = min(q0 + min(QROWS, p.a.R - r * QROWS), p.a.Sq) - 1;
         const bool wraps = q0 + min(QROWS, p.a.R - r * QROWS) > p.a.Sq;
@@ -196,61 +199,79 @@ accumulate_kernel(const TcProblem p, const __grid_constant__ CUtensorMap tmQ, co
             if (2 * rank < halves) tma_load_2d_pair(dst, &tmK, c * 64, r0, bar);
             if (2 * rank + 1 < halves) tma_load_2d_pair(dst + KEY_CHUNK / 2, &tmK, c * 64, r1, bar);
         };
+        const int half_cols = p.n_cols / 2;
+        auto visible = [&](const Walker<ROWS> &v) {
+            if (!ROWS) return true;
+            for (int i = 0; i < v.count; ++i)
+                if (v.sees(v.r_lo + i)) return true;
+            return false;
+        };
         Walker<ROWS> w(p, sh, unit);
-        while (ok && w.next(units)) {
-            const int b = w.b;
-            int page = page_of(b, w.t0, w.n), r0 = 0, r1 = 0;
-            const int half_cols = p.n_cols / 2;
-            if (ROWS) { r0 = row_of(page, w.t0, w.n, 2 * rank); r1 = row_of(page, w.t0, w.n, 2 * rank + 1); }
-            const int halves0 = min(4, (w.n - w.t0 + 63) / 64);
-            auto resident = [&](int c) {
-                if (n_res > 0) ok = ok && mbar_wait(REMPTY(c), (n_res - 1) & 1);
-                if (!ok || !elected) return;
-                const uint32_t dst = smem_u32(res + c * p.res_bytes), bar = rfull_lead + 8u * c;
-                if (rank == 0) mbar_arrive_expect_tx(RFULL(c), ROWS ? halves0 * (KEY_CHUNK / 2) : p.n_cols * 128);
-                if (ROWS) load_keys(r0, r1, halves0, c, dst, bar);
-                else tma_load_2d_pair(dst, &tmQ, c * 64, b * a.R + rank * half_cols, bar);
-            };
-            int c_res = 0;                                                       // resident chunks asked for
-            if (ROWS) {
-                bool any = false;
-                for (int i = 0; i < w.count; ++i) any |= w.sees(w.r_lo + i);
-                if (!any) continue;
-            }
-            for (int i = 0; i < w.count && ok; ++i) {
-                int halves = 0, q_row = 0;
-                if (ROWS) {
-                    if (!w.sees(w.r_lo + i)) continue;
-                    q_row = b * a.R + (w.r_lo + i) * QROWS + rank * half_cols;
-                } else {
-                    const int t0 = w.t0 + i * KEYS;
-                    r0 = row_of(page, t0, w.n, 2 * rank);
-                    r1 = row_of(page, t0, w.n, 2 * rank + 1);
-                    halves = min(4, (w.n - t0 + 63) / 64);
-                    if (i + 1 < w.count) page = page_of(b, t0 + KEYS, w.n);      // the next tile's, ahead of time
-                }
-                for (int c = 0; c < p.chunks && ok; ++c) {
-                    // the resident chunk is asked for one ring length behind the streaming ones: the last MMAs of the previous
-                    // set, which free it, also free the slots
-                    if (c_res <= c && (c >= p.slots || ROWS)) resident(c_res++);
-                    if (use > 0) ok = ok && mbar_wait(EMPTY(s), (use - 1) & 1);
-                    if (ok && elected) {
-                        const uint32_t dst = smem_u32(ring + s * p.slot_bytes), bar = full_lead + 8u * s;
-                        if (ROWS) {
-                            if (rank == 0) mbar_arrive_expect_tx(FULL(s), p.n_cols * 128);
-                            tma_load_2d_pair(dst, &tmQ, c * 64, q_row, bar);
-                        } else {
-                            if (rank == 0) mbar_arrive_expect_tx(FULL(s), halves * (KEY_CHUNK / 2));
-                            load_keys(r0, r1, halves, c, dst, bar);
-                        }
+        bool more = w.next(units);
+        while (ok && more) {
+            Walker<ROWS> after = w;                    // the set behind this one: its resident operand is brought into L2 meanwhile
+            more = after.next(units);
+            if (visible(w)) {
+                const int b = w.b;
+                int page = page_of(b, w.t0, w.n), r0 = 0, r1 = 0;
+                if (ROWS) { r0 = row_of(page, w.t0, w.n, 2 * rank); r1 = row_of(page, w.t0, w.n, 2 * rank + 1); }
+                const int halves0 = min(4, (w.n - w.t0 + 63) / 64);
+                int page_after = 0;
+                if (ROWS && more) page_after = page_of(after.b, after.t0, after.n);
+                bool first = true;
+                for (int i = 0; i < w.count && ok; ++i) {
+                    int halves = 0, q_row = 0;
+                    if (ROWS) {
+                        if (!w.sees(w.r_lo + i)) continue;
+                        q_row = b * a.R + (w.r_lo + i) * QROWS + rank * half_cols;
+                    } else {
+                        const int t0 = w.t0 + i * KEYS;
+                        r0 = row_of(page, t0, w.n, 2 * rank);
+                        r1 = row_of(page, t0, w.n, 2 * rank + 1);
+                        halves = min(4, (w.n - t0 + 63) / 64);
+                        if (i + 1 < w.count) page = page_of(b, t0 + KEYS, w.n);          // the next tile's, ahead of time
                     }
-                    if (++s == p.slots) { s = 0; ++use; }
-                    if (c == min(p.slots, p.chunks) - 1)
-                        while (c_res < p.chunks && c_res <= c) resident(c_res++);
+                    for (int c = 0; c < p.chunks && ok; ++c) {
+                        // chunk c of both operands is freed by the same MMAs of the previous set, and the first MMAs need chunk 0 of both
+                        if (first) {
+                            if (n_res > 0) ok = mbar_wait(REMPTY(c), (n_res - 1) & 1);
+                            if (ok && elected) {
+                                const uint32_t dst = smem_u32(res + c * p.res_bytes), bar = rfull_lead + 8u * c;
+                                if (rank == 0) mbar_arrive_expect_tx(RFULL(c), ROWS ? halves0 * (KEY_CHUNK / 2) : p.n_cols * 128);
+                                if (ROWS) load_keys(r0, r1, halves0, c, dst, bar);
+                                else tma_load_2d_pair(dst, &tmQ, c * 64, b * a.R + rank * half_cols, bar);
+                            }
+                        }
+                        if (use > 0) ok = ok && mbar_wait(EMPTY(s), (use - 1) & 1);
+                        if (ok && elected) {
+                            const uint32_t dst = smem_u32(ring + s * p.slot_bytes), bar = full_lead + 8u * s;
+                            if (ROWS) {
+                                if (rank == 0) mbar_arrive_expect_tx(FULL(s), p.n_cols * 128);
+                                tma_load_2d_pair(dst, &tmQ, c * 64, q_row, bar);
+                            } else {
+                                if (rank == 0) mbar_arrive_expect_tx(FULL(s), halves * (KEY_CHUNK / 2));
+                                load_keys(r0, r1, halves, c, dst, bar);
+                            }
+                        }
+                        if (++s == p.slots) { s = 0; ++use; }
+                    }
+                    if (first && more) {
+                        int n0 = 0, n1 = 0;
+                        if (ROWS) { n0 = row_of(page_after, after.t0, after.n, 2 * rank); n1 = row_of(page_after, after.t0, after.n, 2 * rank + 1); }
+                        if (elected)
+                            for (int c = 0; c < p.chunks; ++c) {
+                                if (ROWS) {
+                                    tma_prefetch_2d(&tmK, c * 64, n0);
+                                    tma_prefetch_2d(&tmK, c * 64, n1);
+                                } else if (after.b != b) tma_prefetch_2d(&tmQ, c * 64, after.b * a.R + rank * half_cols);
+                            }
+                        __syncwarp();
+                    }
+                    first = false;
                 }
-                while (c_res < p.chunks) resident(c_res++);
+                ++n_res;
             }
-            ++n_res;
+            w = after;
         }
         if (!ok && !dead && lane == 0) atomicCAS(&g_acc_error, 0, ERR_PRODUCER);
         __syncwarp();
