@@ -31,14 +31,17 @@ __device__ __forceinline__ float silu(float x) { return x / (1.f + __expf(-x)); 
 // Block (32 experts, one of gridDim.y slices of d, TOK tokens): a lane owns an expert, a warp every 16th of ROWS rows at a time,
 // whose loads are all in flight at once.  part[s, t, e] holds slice s's share of the logit.  All blocks together also clear the
 // counters of the kernel behind.  For one token 512 rows and one block per SM (64 registers, as two blocks would leave, spill and
-// cost 3 us of 23 .. 150); for more 256 rows, 8 tokens and two blocks.
+// cost 3 us of 23 .. 150); for more 128 rows, 8 tokens and two blocks (256 rows
+// spill).
 constexpr int GATE_THREADS = 512, GATE_TOK = 8, MAX_SLICES = 32;
 
 template <typename T, int TOK, int ROWS>
 __global__ void __launch_bounds__(GATE_THREADS, TOK == 1 ? 1 : 2) gate_kernel(const T *__restrict__ x, const float *__restrict__ Wg,
                                                             double *__restrict__ part, unsigned *__restrict__ counters,
                                                             int n_counters, int n_tok, int d, int E) {
-    __shared__ double s_x[ROWS][TOK];                       // later the warps' partial sums
+    // activations as [row][token] (one token of padding against bank conflicts), later the warps' sums as [warp][token][expert]
+    constexpr int LDX = TOK == 1 ? 1 : TOK + 1, WARPS = GATE_THREADS / 32;
+    __shared__ double s_x[ROWS * LDX > WARPS * TOK * 32 ? ROWS * LDX : WARPS * TOK * 32];
     ptx::launch_dependents();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int e = blockIdx.x * 32 + lane, t0 = blockIdx.z * TOK;
@@ -69,7 +72,7 @@ __global__ void __launch_bounds__(GATE_THREADS, TOK == 1 ? 1 : 2) gate_kernel(co
                 v[i] = (r < rows && t0 + j < n_tok) ? to_f32(x[(size_t)(t0 + j) * d + r0 + r]) : 0.f;
             }
 #pragma unroll
-            for (int i = 0; i < ROWS * TOK / GATE_THREADS; ++i) s_x[part0 + i * (GATE_THREADS / TOK)][j] = (double)v[i];
+            for (int i = 0; i < ROWS * TOK / GATE_THREADS; ++i) s_x[(part0 + i * (GATE_THREADS / TOK)) * LDX + j] = (double)v[i];
         }
         __syncthreads();
 #pragma unroll
@@ -78,27 +81,18 @@ __global__ void __launch_bounds__(GATE_THREADS, TOK == 1 ? 1 : 2) gate_kernel(co
             if (r >= rows) break;
             const double wd = (double)wv[i];
 #pragma unroll
-            for (int j = 0; j < TOK; ++j) acc[j] = fma(s_x[r][j], wd, acc[j]);
+            for (int j = 0; j < TOK; ++j) acc[j] = fma(s_x[r * LDX + j], wd, acc[j]);
         }
     }
-    // the warps' sums, half of the warps at a time through the staging buffer: [8 warps][tokens][32 lanes]
-    double *red = &s_x[0][0];
-    for (int step = 8; step > 0; step >>= 1) {
-        __syncthreads();
-        if (warp >= step && warp < 2 * step) {
+    __syncthreads();
 #pragma unroll
-            for (int j = 0; j < TOK; ++j) red[((warp - step) * TOK + j) * 32 + lane] = acc[j];
-        }
-        __syncthreads();
-        if (warp < step) {
+    for (int j = 0; j < TOK; ++j) s_x[(warp * TOK + j) * 32 + lane] = acc[j];
+    __syncthreads();
+    if (warp < TOK && e < E && t0 + warp < n_tok) {          // warp j sums token j
+        double z = 0.0;
 #pragma unroll
-            for (int j = 0; j < TOK; ++j) acc[j] += red[(warp * TOK + j) * 32 + lane];
-        }
-    }
-    if (warp == 0 && e < E) {
-#pragma unroll
-        for (int j = 0; j < TOK; ++j)
-            if (t0 + j < n_tok) part[((size_t)blockIdx.y * n_tok + t0 + j) * E + e] = acc[j];
+        for (int w = 0; w < WARPS; ++w) z += s_x[(w * TOK + warp) * 32 + lane];
+        part[((size_t)blockIdx.y * n_tok + t0 + warp) * E + e] = z;
     }
 }
 
@@ -107,7 +101,7 @@ static int launch_gate(const void *x, const float *Wg, double *part, unsigned *c
                        int slices, cudaStream_t s) {
     const dim3 grid((E + 31) / 32, slices, (n_tok + GATE_TOK - 1) / GATE_TOK);
     if (n_tok == 1) gate_kernel<T, 1, 512><<<grid, GATE_THREADS, 0, s>>>(static_cast<const T *>(x), Wg, part, counters, n_counters, n_tok, d, E);
-    else gate_kernel<T, GATE_TOK, 256><<<grid, GATE_THREADS, 0, s>>>(static_cast<const T *>(x), Wg, part, counters, n_counters, n_tok, d, E);
+    else gate_kernel<T, GATE_TOK, 128><<<grid, GATE_THREADS, 0, s>>>(static_cast<const T *>(x), Wg, part, counters, n_counters, n_tok, d, E);
     return check_launch();
 }
 
