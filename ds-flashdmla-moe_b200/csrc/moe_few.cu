@@ -154,21 +154,28 @@ __device__ __forceinline__ void topk_warp(unsigned long long *key, int E, int k,
     if (lane < k) { idx[lane] = my_i; w[lane] = my_w / sum; }
 }
 
-// Sort keys of one token's logits into key [E]: sums of the slices, in order, eight loads in flight (all 32 at once take 1 us
-// longer for the few slices of a narrow layer and gain nothing for wide ones).  Returns whether this thread saw a NaN.
+// Sort keys of one token's logits into key [E]: sums of the slices, in order, for two experts at a time with eight loads each in
+// flight (32 each take 1 us longer for the few slices of a narrow layer and gain nothing for wide ones).  Returns whether this
+// thread saw a NaN.
 __device__ __forceinline__ bool token_keys(const double *__restrict__ part, int slices, size_t stride, int E, unsigned long long *key) {
     bool nan = false;
-    for (int e = threadIdx.x; e < E; e += blockDim.x) {
-        double z = 0.0;
+    for (int e0 = threadIdx.x; e0 < E; e0 += 2 * blockDim.x) {
+        const int e1 = e0 + blockDim.x < E ? e0 + blockDim.x : e0;
+        double z[2] = {0.0, 0.0};
         for (int s0 = 0; s0 < slices; s0 += 8) {
-            double v[8];
+            double v[2][8];
 #pragma unroll
-            for (int s = 0; s < 8; ++s) v[s] = s0 + s < slices ? part[(size_t)(s0 + s) * stride + e] : 0.0;
+            for (int s = 0; s < 8; ++s) {
+                const double *row = part + (size_t)(s0 + s) * stride;
+                v[0][s] = s0 + s < slices ? row[e0] : 0.0;
+                v[1][s] = s0 + s < slices ? row[e1] : 0.0;
+            }
 #pragma unroll
-            for (int s = 0; s < 8; ++s) z += v[s];
+            for (int s = 0; s < 8; ++s) { z[0] += v[0][s]; z[1] += v[1][s]; }
         }
-        key[e] = logit_key(z);
-        nan |= isnan(z);
+        key[e0] = logit_key(z[0]);
+        key[e1] = logit_key(z[1]);               // the same expert again where there is no second one
+        nan |= isnan(z[0]) || isnan(z[1]);
     }
     return nan;
 }

@@ -97,7 +97,7 @@ __device__ __forceinline__ bool grid_wait(const unsigned *bar, unsigned n) {
     return false;
 }
 
-template <int NP>
+template <int NP, bool LAT>
 __global__ void __launch_bounds__(TC_THREADS, 1)
 layer_kernel(const TcProblem p, const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmH,
              const __grid_constant__ CUtensorMap tmW1, const __grid_constant__ CUtensorMap tmW3, const __grid_constant__ CUtensorMap tmW2,
@@ -488,10 +488,10 @@ layer_kernel(const TcProblem p, const __grid_constant__ CUtensorMap tmX, const _
                 // tiles cut along their reduction: all CTAs sum the pieces, in order, and write h
                 if (L == 0 && !dead && !grid_wait(p.bars + 1, gridDim.x)) atomicCAS(&g_few_error, 0, ERR_GRID);
                 named_bar_sync(1, 128);
-                // one column a thread and all pieces in flight for few tokens (latency), four columns beyond (fewer rounds); not both
-                // in one kernel, whose first launch after other work waits for its instructions
+                // LAT (few rows of h): one column a thread and all its pieces in flight; otherwise four columns a thread.  Two
+                // instantiations, because the first launch after other work waits for its instructions.
                 const unsigned elems = dead ? 0u : (unsigned)p.rows * (unsigned)p.f, threads = gridDim.x * 128;
-                if constexpr (NP == 16) {
+                if constexpr (LAT) {
                     for (unsigned u = blockIdx.x * 128 + L; u < elems; u += threads) {
                         const unsigned r = u / p.f, c = u - r * p.f;
                         const float *o = p.pieces + (size_t)r * 2 * ld1 + c;
@@ -506,28 +506,42 @@ layer_kernel(const TcProblem p, const __grid_constant__ CUtensorMap tmX, const _
                         p.h[u] = __float2bfloat16_rn(silu(x1) * x3);
                     }
                 } else {
-                    for (unsigned u = (blockIdx.x * 128 + L) * 4; u < elems; u += threads * 4) {
-                        const unsigned r = u / p.f, c = u - r * p.f;
-                        const float *o = p.pieces + (size_t)r * 2 * ld1 + c;
-                        float x1[4] = {}, x3[4] = {};
-                        for (unsigned z0 = 0; z0 < it1.split; z0 += 8) {
-                            float4 v1[8], v3[8];
+                    // two groups of four columns at a time, `threads` groups apart, four pieces of both in flight
+                    for (unsigned u0 = (blockIdx.x * 128 + L) * 4; u0 < elems; u0 += threads * 8) {
+                        float x1[2][4] = {}, x3[2][4] = {};
+                        const float *o[2];
 #pragma unroll
-                            for (unsigned z = 0; z < 8; ++z) {
-                                const bool in = z0 + z < it1.split;
-                                const float *q = o + (z0 + z) * slab1;
-                                v1[z] = in ? __ldcg(reinterpret_cast<const float4 *>(q)) : make_float4(0.f, 0.f, 0.f, 0.f);
-                                v3[z] = in ? __ldcg(reinterpret_cast<const float4 *>(q + ld1)) : make_float4(0.f, 0.f, 0.f, 0.f);
-                            }
-#pragma unroll
-                            for (unsigned z = 0; z < 8; ++z) {
-                                x1[0] += v1[z].x; x1[1] += v1[z].y; x1[2] += v1[z].z; x1[3] += v1[z].w;
-                                x3[0] += v3[z].x; x3[1] += v3[z].y; x3[2] += v3[z].z; x3[3] += v3[z].w;
-                            }
+                        for (int g = 0; g < 2; ++g) {
+                            const unsigned u = min(u0 + g * threads * 4, elems - 4), r = u / p.f, c = u - r * p.f;
+                            o[g] = p.pieces + (size_t)r * 2 * ld1 + c;
                         }
-                        const __nv_bfloat162 lo = __floats2bfloat162_rn(silu(x1[0]) * x3[0], silu(x1[1]) * x3[1]),
-                                             hi = __floats2bfloat162_rn(silu(x1[2]) * x3[2], silu(x1[3]) * x3[3]);
-                        *reinterpret_cast<uint2 *>(p.h + u) = make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
+                        for (unsigned z0 = 0; z0 < it1.split; z0 += 4) {
+                            float4 v1[2][4], v3[2][4];
+#pragma unroll
+                            for (int g = 0; g < 2; ++g)
+#pragma unroll
+                                for (unsigned z = 0; z < 4; ++z) {
+                                    const bool in = z0 + z < it1.split;
+                                    const float *q = o[g] + (z0 + z) * slab1;
+                                    v1[g][z] = in ? __ldcg(reinterpret_cast<const float4 *>(q)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                                    v3[g][z] = in ? __ldcg(reinterpret_cast<const float4 *>(q + ld1)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                                }
+#pragma unroll
+                            for (int g = 0; g < 2; ++g)
+#pragma unroll
+                                for (unsigned z = 0; z < 4; ++z) {
+                                    x1[g][0] += v1[g][z].x; x1[g][1] += v1[g][z].y; x1[g][2] += v1[g][z].z; x1[g][3] += v1[g][z].w;
+                                    x3[g][0] += v3[g][z].x; x3[g][1] += v3[g][z].y; x3[g][2] += v3[g][z].z; x3[g][3] += v3[g][z].w;
+                                }
+                        }
+#pragma unroll
+                        for (int g = 0; g < 2; ++g) {
+                            const unsigned u = u0 + g * threads * 4;
+                            if (u >= elems) break;
+                            const __nv_bfloat162 lo = __floats2bfloat162_rn(silu(x1[g][0]) * x3[g][0], silu(x1[g][1]) * x3[g][1]),
+                                                 hi = __floats2bfloat162_rn(silu(x1[g][2]) * x3[g][2], silu(x1[g][3]) * x3[g][3]);
+                            *reinterpret_cast<uint2 *>(p.h + u) = make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
+                        }
                     }
                 }
                 arrive(3);
@@ -545,9 +559,9 @@ layer_kernel(const TcProblem p, const __grid_constant__ CUtensorMap tmX, const _
     const size_t slab = (size_t)p.rows * p.d;
     const int n = p.k + p.shared;
     const long long threads = (long long)gridDim.x * TC_THREADS, me = (long long)blockIdx.x * TC_THREADS + tid;
-    // V columns a thread (one for few tokens, four beyond), Z pieces each of J choices in flight
-    auto weighted_sum = [&](auto v_, auto j_) {
-        constexpr int V = decltype(v_)::value, J = decltype(j_)::value, Z = 4;
+    // V columns a thread, Z pieces each of nine choices (eight and the shared expert) in flight
+    auto weighted_sum = [&](auto v_, auto z_) {
+        constexpr int V = decltype(v_)::value, Z = decltype(z_)::value, J = 9;
         const int per_row = p.d / V;
         for (long long u = me; u < (long long)p.n_tok * per_row; u += threads) {
             const int t = (int)(u / per_row), c = (int)(u - (long long)t * per_row) * V;
@@ -591,8 +605,8 @@ layer_kernel(const TcProblem p, const __grid_constant__ CUtensorMap tmX, const _
             } else *o = __float2bfloat16_rn(sum[0]);
         }
     };
-    if constexpr (NP == 16) weighted_sum(std::integral_constant<int, 1>{}, std::integral_constant<int, 9>{});
-    else weighted_sum(std::integral_constant<int, 4>{}, std::integral_constant<int, 4>{});
+    if constexpr (LAT) weighted_sum(std::integral_constant<int, 1>{}, std::integral_constant<int, 4>{});
+    else weighted_sum(std::integral_constant<int, 4>{}, std::integral_constant<int, 2>{});
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------------
@@ -638,7 +652,7 @@ static bool tc_aligned(const Args &a) {
              reinterpret_cast<uintptr_t>(a.S2)) & 15) == 0 && (reinterpret_cast<uintptr_t>(a.out) & 7) == 0;
 }
 
-template <int NP>
+template <int NP, bool LAT>
 static int launch_layer(const TcProblem &p, const Args &a, int grid, cudaStream_t s) {
     CUtensorMap tmX, tmH, tm[6];
     if (!make_tensor_map_bf16(&tmX, a.x, a.n_tok, a.d, NP) ||
@@ -649,10 +663,7 @@ static int launch_layer(const TcProblem &p, const Args &a, int grid, cudaStream_
         const long long rows = (i % 3 == 2 ? a.f : a.d) * (long long)(i < 3 ? a.E : 1);
         if (!make_tensor_map_bf16_chunked(&tm[i], base[i], rows, i % 3 == 2 ? a.d : a.f, 64, 2)) return FDMLA_ERR_CUDA;
     }
-    if (cudaFuncSetAttribute(layer_kernel<NP>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<NP>::SMEM) != cudaSuccess) {
-        cudaGetLastError();
-        return FDMLA_ERR_CUDA;
-    }
+    if (!allow_smem<layer_kernel<NP, LAT>>(Cfg<NP>::SMEM)) return FDMLA_ERR_CUDA;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)grid);
     cfg.blockDim = dim3(TC_THREADS);
@@ -665,7 +676,7 @@ static int launch_layer(const TcProblem &p, const Args &a, int grid, cudaStream_
     at[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
     cfg.numAttrs = 2;
-    if (cudaLaunchKernelEx(&cfg, layer_kernel<NP>, p, tmX, tmH, tm[0], tm[1], tm[2], tm[3], tm[4], tm[5]) != cudaSuccess) {
+    if (cudaLaunchKernelEx(&cfg, layer_kernel<NP, LAT>, p, tmX, tmH, tm[0], tm[1], tm[2], tm[3], tm[4], tm[5]) != cudaSuccess) {
         cudaGetLastError();
         return FDMLA_ERR_CUDA;
     }
@@ -689,10 +700,12 @@ static int run_tensor(const Args &a, uint8_t *ws, cudaStream_t s) {
     p.pieces = reinterpret_cast<float *>(ws + L.pieces);
     p.out = static_cast<__nv_bfloat16 *>(a.out);
     if (launch_gate<__nv_bfloat16>(a.x, a.Wg, part, counters, N_COUNTERS, a.n_tok, a.d, a.E, p.slices, s) != FDMLA_OK) return FDMLA_ERR_CUDA;
-    if (a.n_tok <= 16) return launch_layer<16>(p, a, L.grid, s);
-    if (a.n_tok <= 32) return launch_layer<32>(p, a, L.grid, s);
-    if (a.n_tok <= 64) return launch_layer<64>(p, a, L.grid, s);
-    return launch_layer<128>(p, a, L.grid, s);
+    // one column a thread in the sums of pieces while that is at most two rounds over the grid
+    if (a.n_tok <= 16)
+        return (long long)p.rows * a.f <= 256LL * L.grid ? launch_layer<16, true>(p, a, L.grid, s) : launch_layer<16, false>(p, a, L.grid, s);
+    if (a.n_tok <= 32) return launch_layer<32, false>(p, a, L.grid, s);
+    if (a.n_tok <= 64) return launch_layer<64, false>(p, a, L.grid, s);
+    return launch_layer<128, false>(p, a, L.grid, s);
 }
 
 }  // namespace few
