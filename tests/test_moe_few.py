@@ -219,6 +219,19 @@ def test_layer_object_strides_streams_and_graph(cuda):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, layer.forward_few(src))
+    # two calls side by side inside one graph
+    fork, outs = torch.cuda.CUDAGraph(), [torch.empty_like(y) for _ in range(2)]
+    with torch.cuda.graph(fork):
+        cur = torch.cuda.current_stream()
+        s1.wait_stream(cur)
+        with torch.cuda.stream(s1):
+            layer.forward_few(xin, outs[0])
+        layer.forward_few(xin, outs[1])
+        cur.wait_stream(s1)
+    for _ in range(5):
+        fork.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], y) and torch.equal(outs[1], y)
     assert layer.forward_few(xt[:0]).shape == (0, 256)
     with pytest.raises(FlashDMLAError):
         layer.forward_few(torch.zeros(129, 256, dtype=torch.bfloat16, device=cuda))
