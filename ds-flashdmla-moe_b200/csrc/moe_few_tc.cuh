@@ -139,7 +139,8 @@ layer_kernel(const TcProblem p, const __grid_constant__ CUtensorMap tmX, const _
     // which tokens chose an expert: a 128-bit mask each
     uint32_t(*s_mask)[4] = reinterpret_cast<uint32_t(*)[4]>(ring + 16384);
     uint16_t *s_first = reinterpret_cast<uint16_t *>(ring + 16384 + MAX_E * 16), *s_idx = s_first + MAX_E;
-    for (int i = tid; i < p.E * 4; i += TC_THREADS) (&s_mask[0][0])[i] = 0u;
+    if (!single)
+        for (int i = tid; i < p.E * 4; i += TC_THREADS) (&s_mask[0][0])[i] = 0u;
     if (tid == 0 && !sh.dead && !single) {
         red_release_gpu(p.bars);
         if (!grid_wait(p.bars, gridDim.x)) { sh.dead = 1; atomicCAS(&g_few_error, 0, ERR_GRID); }
@@ -150,64 +151,80 @@ layer_kernel(const TcProblem p, const __grid_constant__ CUtensorMap tmX, const _
     const uint32_t tmem = sh.tmem;
     const bool dead = sh.dead != 0;
     // ---- routed experts in ascending order, their rows of h in token order (the same in every CTA) -------------------------------
-    if (!dead)
-        for (int i = tid; i < choices; i += TC_THREADS) {
-            const int e = single ? sh.idx[i] : __ldcg(p.idx + i), t = i / p.k;
-            s_idx[i] = (uint16_t)e;
-            atomicOr(&s_mask[e][t >> 5], 1u << (t & 31));
+    if (single) {                                      // the winners' ranks, without masks
+        if (tid < p.k) {
+            const int e = sh.idx[tid];
+            int r = 0;
+            for (int j = 0; j < p.k; ++j) r += sh.idx[j] < e;
+            sh.expert[r] = (uint16_t)e;
+            sh.first[r] = sh.group[r] = sh.row[tid] = (uint16_t)r;
+            sh.token[r] = 0;
         }
-    __syncthreads();
-    {   // a thread owns `per` neighbouring experts; prefix sums of (experts, groups) and rows over the block
-        const int per = (p.E + TC_THREADS - 1) / TC_THREADS, e0 = min(tid * per, p.E), e1 = min(e0 + per, p.E);
-        auto tokens = [&](int e) { return __popc(s_mask[e][0]) + __popc(s_mask[e][1]) + __popc(s_mask[e][2]) + __popc(s_mask[e][3]); };
-        uint32_t cnt = 0, rows = 0;                    // experts | groups << 16
-        for (int e = e0; e < e1; ++e) {
-            const int n = tokens(e);
-            cnt += (n > 0 ? 0x10001u : 0u) + (n > GROUP ? 0x10000u : 0u);
-            rows += n;
+        if (tid == 0) {
+            sh.first[p.k] = sh.group[p.k] = (uint16_t)p.k;             // the shared expert's group, if there is one
+            sh.n_routed = p.k;
+            sh.n_groups = p.k + p.shared;
         }
-        uint32_t ci = cnt, ri = rows;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const uint32_t cu = __shfl_up_sync(0xffffffffu, ci, o), ru = __shfl_up_sync(0xffffffffu, ri, o);
-            if (lane >= o) { ci += cu; ri += ru; }
-        }
-        if (lane == 31) { sh.scan[warp] = ci; sh.scan[8 + warp] = ri; }
-        __syncthreads();
-        for (int v = 0; v < warp; ++v) { ci += sh.scan[v]; ri += sh.scan[8 + v]; }
-        uint32_t c = ci - cnt, r = ri - rows;
-        for (int e = e0; e < e1; ++e) {
-            const int n = tokens(e);
-            if (n == 0) continue;
-            const uint32_t a = c & 0xffffu, g = c >> 16;
-            sh.expert[a] = (uint16_t)e;
-            sh.first[a] = s_first[e] = (uint16_t)r;
-            sh.group[g] = (uint16_t)a;
-            if (n > GROUP) sh.group[g + 1] = (uint16_t)(a | 0x8000);
-            c += 0x10001u + (n > GROUP ? 0x10000u : 0u);
-            r += n;
-        }
-        if (tid == TC_THREADS - 1) {
-            int n_grp = ci >> 16;
-            sh.n_routed = ci & 0xffffu;
-            sh.first[sh.n_routed] = (uint16_t)ri;
-            if (p.shared) {
-                sh.group[n_grp++] = (uint16_t)sh.n_routed;
-                if (p.n_tok > GROUP) sh.group[n_grp++] = (uint16_t)(sh.n_routed | 0x8000);
+    } else {
+        if (!dead)
+            for (int i = tid; i < choices; i += TC_THREADS) {
+                const int e = __ldcg(p.idx + i), t = i / p.k;
+                s_idx[i] = (uint16_t)e;
+                atomicOr(&s_mask[e][t >> 5], 1u << (t & 31));
             }
-            sh.n_groups = n_grp;
+        __syncthreads();
+        {   // a thread owns `per` neighbouring experts; prefix sums of (experts, groups) and rows over the block
+            const int per = (p.E + TC_THREADS - 1) / TC_THREADS, e0 = min(tid * per, p.E), e1 = min(e0 + per, p.E);
+            auto tokens = [&](int e) { return __popc(s_mask[e][0]) + __popc(s_mask[e][1]) + __popc(s_mask[e][2]) + __popc(s_mask[e][3]); };
+            uint32_t cnt = 0, rows = 0;                    // experts | groups << 16
+            for (int e = e0; e < e1; ++e) {
+                const int n = tokens(e);
+                cnt += (n > 0 ? 0x10001u : 0u) + (n > GROUP ? 0x10000u : 0u);
+                rows += n;
+            }
+            uint32_t ci = cnt, ri = rows;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t cu = __shfl_up_sync(0xffffffffu, ci, o), ru = __shfl_up_sync(0xffffffffu, ri, o);
+                if (lane >= o) { ci += cu; ri += ru; }
+            }
+            if (lane == 31) { sh.scan[warp] = ci; sh.scan[8 + warp] = ri; }
+            __syncthreads();
+            for (int v = 0; v < warp; ++v) { ci += sh.scan[v]; ri += sh.scan[8 + v]; }
+            uint32_t c = ci - cnt, r = ri - rows;
+            for (int e = e0; e < e1; ++e) {
+                const int n = tokens(e);
+                if (n == 0) continue;
+                const uint32_t a = c & 0xffffu, g = c >> 16;
+                sh.expert[a] = (uint16_t)e;
+                sh.first[a] = s_first[e] = (uint16_t)r;
+                sh.group[g] = (uint16_t)a;
+                if (n > GROUP) sh.group[g + 1] = (uint16_t)(a | 0x8000);
+                c += 0x10001u + (n > GROUP ? 0x10000u : 0u);
+                r += n;
+            }
+            if (tid == TC_THREADS - 1) {
+                int n_grp = ci >> 16;
+                sh.n_routed = ci & 0xffffu;
+                sh.first[sh.n_routed] = (uint16_t)ri;
+                if (p.shared) {
+                    sh.group[n_grp++] = (uint16_t)sh.n_routed;
+                    if (p.n_tok > GROUP) sh.group[n_grp++] = (uint16_t)(sh.n_routed | 0x8000);
+                }
+                sh.n_groups = n_grp;
+            }
         }
+        __syncthreads();
+        if (!dead)
+            for (int i = tid; i < choices; i += TC_THREADS) {
+                const int e = s_idx[i], t = i / p.k;
+                int r = s_first[e];
+                for (int q = 0; q < t >> 5; ++q) r += __popc(s_mask[e][q]);
+                r += __popc(s_mask[e][t >> 5] & ((1u << (t & 31)) - 1u));
+                sh.row[i] = (uint16_t)r;
+                sh.token[r] = (uint8_t)t;
+            }
     }
-    __syncthreads();
-    if (!dead)
-        for (int i = tid; i < choices; i += TC_THREADS) {
-            const int e = s_idx[i], t = i / p.k;
-            int r = s_first[e];
-            for (int q = 0; q < t >> 5; ++q) r += __popc(s_mask[e][q]);
-            r += __popc(s_mask[e][t >> 5] & ((1u << (t & 31)) - 1u));
-            sh.row[i] = (uint16_t)r;
-            sh.token[r] = (uint8_t)t;
-        }
     fence_proxy_async_all();                           // the copies write where the masks were
     __syncthreads();
     const unsigned routed = sh.n_routed;
