@@ -52,6 +52,8 @@ struct AccProblem {
 
 // ---- accumulate on CUDA cores: any type and width ---------------------------------------------------------------------------
 // Block: 32 keys of one sequence (a lane owns a key, its row in shared memory) x all query rows, four rows per warp at a time.
+// Bound by shared memory and the broadcast loads of the queries, five loads to four multiply-adds: 12.6 TFLOP/s in bf16 at
+// 128 sequences of 4096 keys and 128 heads (6.15 ms).
 constexpr int ACC_WARPS = 8, ACC_ROWS = 4;
 
 template <typename T>
@@ -122,6 +124,7 @@ __global__ void __launch_bounds__(128) stamp_kernel(float *__restrict__ weights,
 // CTAs costs about 1 us, so there are five: a histogram of its own for every round (nobody waits before clearing one), the
 // counts of equal keys from the last round's, evicted and moving rows counted together.  Reading all 2048 bins of 16 CTAs took
 // 6 us a round; now every CTA reads their 64 sums of 32 bins, then the 32 bins of the one that matters: 131072 rows 40 -> 23 us.
+// Bound by latency: 14 us for 128 sequences of 4096 rows (one CTA each: keys 3, rounds 3, ranks and lists 6).
 constexpr int SEL_THREADS = 1024, SEL_WARPS = SEL_THREADS / 32, BINS = 2048, MAX_CLUSTER = 16;
 constexpr int MAX_SEG = 49152;                   // rows per CTA: 192 KB of keys
 
@@ -351,7 +354,7 @@ __global__ void __launch_bounds__(SEL_THREADS, 1) select_kernel(const SelectProb
 
 // ---- evict, part 2: the copies -----------------------------------------------------------------------------------------------
 // A warp takes `span` places (up to 32, fewer when there are few), reads what goes there (kept) and copies the rows that change
-// place, two at a time with three vectors of each in flight per lane (a row of 1152 bytes is 72 vectors of 16; four rows at a
+// place (5.8 TB/s read and written at 135 000 rows of 1152 bytes), two at a time with three vectors of each in flight per lane (a row of 1152 bytes is 72 vectors of 16; four rows at a
 // time take more registers and were 5 % slower).  Rows are read and written once: streaming loads and stores.
 template <typename V>
 __global__ void __launch_bounds__(256) move_kernel(uint8_t *__restrict__ pool, float *__restrict__ weights,

@@ -10,7 +10,8 @@
 // The logits are summed in 64 bits, so which experts win does not depend on the order of a sum (two logits that differ by a
 // rounding of a 32-bit sum would otherwise pick different experts in different kernels).
 //
-// Bound: the weights of the experts that win, 6 d f bytes each, read once for all tokens.
+// Bound: the weights of the experts that win, 6 d f bytes each, read once for all tokens.  One launch of the gate kernel and one of
+// the layer kernel (moe_few_tc.cuh) for bf16 and widths that are multiples of 64, five launches on CUDA cores for the rest.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -217,7 +218,9 @@ __device__ __forceinline__ int expert_rows(const int32_t *idx, int e, int E, int
     return *s_n;
 }
 
-// Block: 64 output columns of one expert, four slices of the reduction, four tokens at a time.
+// Block: 64 output columns of one expert, four slices of the reduction, four tokens at a time.  Reads an expert's weights once per
+// four of its tokens with two bytes per lane and load: bound by the latency of those loads (the layer at T = 1, d = 7168, E = 256,
+// f = 2048 in bf16: 1.44 ms, 0.55 TB/s).
 constexpr int SIMT_COLS = 64, SIMT_TOK = 4;
 
 // UP: h[row, c] = silu(x W1) (x W3);  otherwise: y[row, c] = h W2

@@ -17,6 +17,10 @@
 //
 // Warp 0 issues the copies, warp 1 the MMAs, warps 2-5 read the accumulators (thread = weight column).  All waits are bounded
 // (codes 41-44 of fdmla_device_error_flag).
+//
+// Measured with the gate kernel, replayed from a CUDA graph, d = 7168, f = 2048, E = 256, top-8 and a shared expert: T = 1 147 us
+// (793 MB, 5.4 TB/s), T = 128 3.34 ms (22.3 GB, 6.7 TB/s); d = 4096, f = 1024, E = 64: T = 1 62 us, T = 64 288 us (5.7 TB/s).
+// A step that is not bandwidth: gate 6 us, top-k and tables 6 us, 2 us per grid barrier.
 #pragma once
 
 #include <type_traits>

@@ -18,7 +18,9 @@ With track_weights=True the cache can be bounded: beside every row it keeps the 
     cache.evict(slots, keep=4096, recent=128)   # at most 4096 rows each: the newest 128 and the heaviest others
 
 gives the pages behind row `keep` back.  Rows are then no longer in the order of their tokens (the attention does not
-depend on it); `position(slot)` is the position of the next token, `length(slot)` the number of rows held.
+depend on it); `position(slot)` is the position of the next token, `length(slot)` the number of rows held.  A prompt's
+rows start with weight 0: `ops.accumulate_weights(Q, cache.pool, *cache.tables(slots), m, l, cache.weights)` adds what the
+prompt's own queries (or its last ones) gave them.
 
 Page bookkeeping (free list, lengths, the host copy of the page table) is plain Python and
 runs without a GPU (`device="cpu"`: the pool then only exists as metadata and `append`
