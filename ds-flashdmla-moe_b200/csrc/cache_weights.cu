@@ -507,14 +507,14 @@ extern "C" int fdmla_cache_evict(void *kv_pool, float *weights, int32_t *positio
     if (B == 0) return FDMLA_OK;
     if (!kv_pool || !weights || !positions || !page_table || !seqlens || !next_position || !kept || !new_seqlens) return FDMLA_ERR_INVALID;
     if (!pages_ok(B, page_size, max_pages, num_pages) || keep > (1 << 30)) return FDMLA_ERR_UNSUPPORTED;
-    if (max_pages > 0 && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 3) || workspace_bytes < fdmla_cache_evict_workspace_bytes(B, keep, page_size, max_pages))) return FDMLA_ERR_WORKSPACE;
     cudaStream_t s = (cudaStream_t)stream;
     const int cap = page_size * max_pages;
+    if (cap > cw::MAX_CLUSTER * (cw::MAX_SEG - 32)) return FDMLA_ERR_UNSUPPORTED;
     // CTAs per sequence: enough for every SM as long as a CTA keeps a few thousand rows, and room for the keys of the longest
     int cs = 1;
     while (cs < cw::MAX_CLUSTER && ((cap + cs - 1) / cs > cw::MAX_SEG - 32 || ((long long)B * cs * 2 <= kNumSMs && cap / cs > 4096))) cs *= 2;
-    const int seg = (((cap + cs - 1) / cs) + 31) & ~31;
-    if (seg > cw::MAX_SEG) return FDMLA_ERR_UNSUPPORTED;
+    const int seg = (((cap + cs - 1) / cs) + 31) & ~31;                       // at most MAX_SEG
+    if (max_pages > 0 && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 3) || workspace_bytes < fdmla_cache_evict_workspace_bytes(B, keep, page_size, max_pages))) return FDMLA_ERR_WORKSPACE;
     cw::SelectProblem p{};
     p.weights = weights; p.positions = positions;
     p.pg = cw::Pages{page_table, seqlens, page_size, max_pages, num_pages};

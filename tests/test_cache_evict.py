@@ -116,6 +116,8 @@ def test_c_entry_points_refuse_bad_arguments():
     assert ev(*(1,) * 9, 1 << 20, 1, 4, 5, 576, 64, 4, 4, 1, None) == -1                       # recent > keep
     assert ev(*(1,) * 9, 15, 1, 4, 0, 576, 64, 4, 4, 1, None) == -4                            # workspace
     assert ev(*(1,) * 9, 1 << 30, 1, 4, 0, 576, 64, 20000, 4, 1, None) == -2                   # too many rows per sequence
+    assert ev(*(1,) * 9, 1 << 30, 1, 4, 0, 576, 1, 2 ** 31 - 1, 4, 1, None) == -2
+    assert ev(*(256,) * 9, 1 << 30, 1, 2 ** 30 + 1, 0, 576, 64, 4, 4, 1, None) == -2
     assert L.fdmla_cache_evict_workspace_bytes(3, 100, 64, 1) == 2 * 3 * 64 * 4
     assert L.fdmla_cache_stamp(None, None, None, None, None, 0, 1, 64, 4, 4, None) == 0
     assert L.fdmla_cache_stamp(None, None, None, None, None, 1, 1, 64, 4, 4, None) == -1
