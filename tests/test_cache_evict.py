@@ -293,6 +293,10 @@ ACC_CASES = [
     ([500, 130, 7], 8, 33, 576, 64, torch.bfloat16),          # a window of queries, longer than the last sequence
     ([260], 128, 9, 64, 64, torch.bfloat16),
     ([90, 200], 3, 200, 128, 64, torch.bfloat16),
+    ([500, 130, 3, 256], 8, 4, 576, 64, torch.bfloat16),      # a few queries of a few heads: one tile of query rows, masked
+    ([300, 257, 15], 16, 16, 192, 64, torch.bfloat16),        # exactly one tile
+    ([300, 2000], 1, 257, 64, 64, torch.bfloat16),            # one row more
+    ([1500, 640, 0, 31], 128, 3, 576, 192, torch.bfloat16),   # pages that end inside a tile
     ([300, 20, 0], 8, 1, 160, 16, torch.float32),
     ([70, 33], 5, 4, 24, 48, torch.float32),
     ([70, 33], 5, 4, 31, 5, torch.bfloat16),                  # odd width and page
