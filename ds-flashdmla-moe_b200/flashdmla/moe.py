@@ -140,7 +140,7 @@ def moe_few(x: torch.Tensor, Wg: torch.Tensor, W1: torch.Tensor, W3: torch.Tenso
     x, Wg, W1, W3, W2 = x.contiguous(), Wg.contiguous(), W1.contiguous(), W3.contiguous(), W2.contiguous()
     code = _dtype_code(x)
     if out is None:
-        out = torch.empty(T, d, dtype=dt, device=x.device)
+        out = torch.empty_like(x)
     elif out.shape != (T, d) or out.dtype != dt or out.device != x.device or not out.is_contiguous():
         raise FlashDMLAError("out must be a contiguous [T,d] tensor of x's dtype on its GPU")
     ctx, stream = _launch_on(x)

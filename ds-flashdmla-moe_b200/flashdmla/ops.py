@@ -30,16 +30,17 @@ def _dtype_code(t: torch.Tensor) -> int:
 
 
 def _need_cuda(*ts: torch.Tensor) -> None:
-    dev = None
+    dev = -1
     for t in ts:
         if t is None:
             continue
-        if not t.is_cuda:
+        d = t.get_device() if t.is_cuda else -1
+        if d < 0:
             raise FlashDMLAError("Flash-DMLA operators need CUDA tensors (no CPU fallback)")
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise FlashDMLAError("all tensors must live on the same GPU")
+        if d != dev:
+            if dev >= 0:
+                raise FlashDMLAError("all tensors must live on the same GPU")
+            dev = d
 
 
 def _stream(t: torch.Tensor) -> int:
@@ -53,7 +54,7 @@ _current = contextlib.nullcontext()
 def _launch_on(t: torch.Tensor):
     """(context, stream) for a launch on t's GPU.  Where a call takes ten microseconds on the GPU, entering a device that is
     current already and building a Stream object would take the host half as long."""
-    dev = t.device.index
+    dev = t.get_device()
     ctx = _current if dev == torch.cuda.current_device() else torch.cuda.device(dev)
     return ctx, _raw_stream(dev) if _raw_stream is not None else _stream(t)
 
@@ -528,16 +529,15 @@ def cache_evict(kv_pool, weights, positions, page_table, seqlens, next_position,
     if keep < 1 or not 0 <= recent <= keep:
         raise FlashDMLAError("cache_evict needs keep >= 1 and 0 <= recent <= keep")
     num_pages, page_size, d_qk = kv_pool.shape
-    max_pages, dev = page_table.shape[1], kv_pool.device
+    max_pages = page_table.shape[1]
     page_table, seqlens, next_position = page_table.contiguous(), seqlens.contiguous(), next_position.contiguous()
     code = _dtype_code(kv_pool)
-    kept = torch.empty(B, keep, dtype=torch.int32, device=dev)
-    new_seqlens = torch.empty(B, dtype=torch.int32, device=dev)
+    kept, new_seqlens = seqlens.new_empty((B, keep)), seqlens.new_empty((B,))
     ctx, stream = _launch_on(kv_pool)
     with ctx:
         L = _lib.lib()
         nbytes = L.fdmla_cache_evict_workspace_bytes(B, keep, page_size, max_pages)
-        ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
+        ws = seqlens.new_empty(((max(nbytes, 16) + 3) // 4,))
         check(L.fdmla_cache_evict(kv_pool.data_ptr(), weights.data_ptr(), positions.data_ptr(), page_table.data_ptr(),
                                   seqlens.data_ptr(), next_position.data_ptr(), kept.data_ptr(), new_seqlens.data_ptr(),
                                   ws.data_ptr(), max(nbytes, 16), B, keep, recent, d_qk, page_size, max_pages, num_pages, code,
