@@ -41,7 +41,7 @@ struct TcShared {                                    // in front of the operands
     uint64_t bars[2 * MAX_SLOTS + 2 * MAX_CHUNKS + 4];
     uint32_t tmem;
     int dead, b0, tile0, n_tiles, scan[TC_THREADS / 32];
-    alignas(16) float2 ml[2][QROWS];                             // m log2(e) and 1 / l of the tile's query rows
+    alignas(16) float2 ml[2][QROWS];                 // m log2(e) and 1 / l of the tile's query rows
     int last[2][QROWS];                              // last key each of them sees
 };
 
@@ -215,7 +215,8 @@ accumulate_kernel(const TcProblem p, const __grid_constant__ CUtensorMap tmQ, co
         while (ok && more) {
             Walker<ROWS> after = w;                    // the set behind this one: its resident operand is brought into L2 meanwhile
             more = after.next(units);
-            if (visible(w)) {
+            if (ROWS) ok = __all_sync(0xffffffffu, ok);
+            if (visible(w) && ok) {
                 const int b = w.b;
                 int page = page_of(b, w.t0, w.n), r0 = 0, r1 = 0;
                 if (ROWS) { r0 = row_of(page, w.t0, w.n, 2 * rank); r1 = row_of(page, w.t0, w.n, 2 * rank + 1); }
@@ -259,6 +260,7 @@ accumulate_kernel(const TcProblem p, const __grid_constant__ CUtensorMap tmQ, co
                         }
                         if (++s == p.slots) { s = 0; ++use; }
                     }
+                    if (!ROWS || first) ok = __all_sync(0xffffffffu, ok);        // the lanes exchange page ids below
                     if (first && more) {
                         int n0 = 0, n1 = 0;
                         if (ROWS) { n0 = row_of(page_after, after.t0, after.n, 2 * rank); n1 = row_of(page_after, after.t0, after.n, 2 * rank + 1); }

@@ -252,7 +252,7 @@ layer_kernel(const TcProblem p, const __grid_constant__ CUtensorMap tmX, const _
         // ================================ producer ================================
         const bool elected = elect_one();
         if (lane == 0) { prefetch_tmap(&tmX); prefetch_tmap(&tmW1); prefetch_tmap(&tmW3); prefetch_tmap(&tmW2); prefetch_tmap(&tmH); }
-        bool ok = !dead;
+        bool ok = !dead;                               // the same in every lane: the lanes exchange values below
         int s = 0, use = 0, n_items = 0;
         // the next item is asked for while the current one is loaded; the counter's first answer is item gridDim.x
         auto ask = [&](int stage, unsigned taken) { return lane == 0 ? taken + atomicAdd(p.next + stage - 1, 1u) : 0u; };
@@ -272,7 +272,7 @@ layer_kernel(const TcProblem p, const __grid_constant__ CUtensorMap tmX, const _
             const CUtensorMap *m1 = own ? &tmS1 : &tmW1, *m3 = own ? &tmS3 : &tmW3;
             const int row0 = own ? 0 : (int)sh.expert[a] * p.d;
             for (unsigned kc = it1.begin(ks); kc < it1.begin(ks + 1) && ok; ++kc) {
-                if (use > 0) ok = mbar_wait(EMPTY(s), (use - 1) & 1);
+                if (use > 0) ok = __all_sync(0xffffffffu, mbar_wait(EMPTY(s), (use - 1) & 1));
                 if (ok && elected) {
                     const uint32_t dst = smem_u32(ring + s * STAGE);
                     mbar_arrive_expect_tx(FULL(s), A_BYTES + NP * 128);
@@ -349,7 +349,7 @@ layer_kernel(const TcProblem p, const __grid_constant__ CUtensorMap tmX, const _
                     __syncwarp();
                     pass();
                 }
-                if (ok && use > 0) ok = mbar_wait(EMPTY(s), (use - 1) & 1);
+                if (ok && use > 0) ok = __all_sync(0xffffffffu, mbar_wait(EMPTY(s), (use - 1) & 1));
                 if (ok && elected) {
                     weights(a, j, c2, n16, s);
                     if (open) acts(row0, c2, n16, s);
