@@ -145,6 +145,13 @@ int fdmla_device_error_flag(int reset) {
               xch = exchange_error_flag(reset), few = few_error_flag(reset), cache = cache_error_flag(reset);
     return fwd ? fwd : (bwd ? bwd : (gemm ? gemm : (xch ? xch : (few ? few : cache))));
 }
+int fdmla_set_device_error_flag(int code) {
+    const bool few = code >= 41 && code <= 44, acc = code >= 51 && code <= 53;
+    if (!few && !acc) return FDMLA_ERR_INVALID;
+    if (few ? few_set_error(code) : cache_set_error(code)) return FDMLA_OK;
+    cudaGetLastError();
+    return FDMLA_ERR_CUDA;
+}
 
 size_t fdmla_exchange_bytes(int world, long long rows, int d_v) { return exchange_bytes(world, rows, d_v); }
 

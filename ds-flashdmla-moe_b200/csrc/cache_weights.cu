@@ -427,6 +427,7 @@ int cache_error_flag(int reset) {
     }
     return wait ? wait : page;
 }
+bool cache_set_error(int code) { return cudaMemcpyToSymbol(cw::g_acc_error, &code, sizeof(int)) == cudaSuccess; }
 
 }  // namespace fdmla
 

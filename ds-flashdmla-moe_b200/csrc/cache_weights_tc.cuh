@@ -445,12 +445,13 @@ accumulate_kernel(const TcProblem p, const __grid_constant__ CUtensorMap tmQ, co
     if (warp == 1) { tc_fence_after_sync(); tmem_dealloc_2cta(tmem, 2 * QROWS); }
 }
 
-// weights += the splits' partial sums, in order
+// weights += the splits' partial sums, in order.  After a time-out (of the launch in front or an earlier one) the partial sums were
+// not all written: nothing is added.
 __global__ void __launch_bounds__(256) add_partials_kernel(const float *__restrict__ partial, float *__restrict__ weights, const Pages pg,
                                                            int B, int splits) {
     const int b = blockIdx.y, t = blockIdx.x * 256 + threadIdx.x;
     const size_t cap = (size_t)pg.max_pages * pg.page_size;
-    if (t >= pg.length(b)) return;
+    if (t >= pg.length(b) || *reinterpret_cast<volatile int *>(&g_acc_error) != 0) return;
     float g = 0.f;
     for (int s = 0; s < splits; ++s) g += partial[((size_t)s * B + b) * cap + t];
     const long long row = pg.row(b, t);

@@ -148,6 +148,9 @@ int gemm_error_flag(int reset);
 int exchange_error_flag(int reset);
 int few_error_flag(int reset);            // time-outs of the few-token MoE kernel
 int cache_error_flag(int reset);          // bad page ids and lengths seen by the cache-weight kernels
+// the flags set from the host, as a wait that gave up would set them
+bool few_set_error(int code);
+bool cache_set_error(int code);
 size_t exchange_bytes(int world, long long rows, int d_v);
 int launch_exchange_merge(const float *O_part, const float *m_part, const float *l_part, int num_parts, void *msg,
                           void *const *bufs, int world, int rank, long long rows, int d_v, void *O,

@@ -740,5 +740,6 @@ int few_error_flag(int reset) {
     }
     return v;
 }
+bool few_set_error(int code) { return cudaMemcpyToSymbol(few::g_few_error, &code, sizeof(int)) == cudaSuccess; }
 
 }  // namespace fdmla

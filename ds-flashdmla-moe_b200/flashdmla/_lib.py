@@ -27,6 +27,7 @@ SIGNATURES = {
     "fdmla_set_single_cta": (_i, [_i]),
     "fdmla_last_kernel": (ctypes.c_char_p, []),
     "fdmla_device_error_flag": (_i, [_i]),
+    "fdmla_set_device_error_flag": (_i, [_i]),
     "fdmla_fwd_cache_latent": (_i, [_vp] * 5 + [_i] * 6 + [_f, _i, _i, _vp]),
     "fdmla_fwd_on_the_fly_workspace_bytes": (_sz, [_i] * 5),
     "fdmla_fwd_on_the_fly": (_i, [_vp] * 9 + [_sz] + [_i] * 6 + [_f, _i, _i, _vp]),

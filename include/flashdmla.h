@@ -84,6 +84,10 @@ const char *fdmla_last_kernel(void);
  * launches.  No reference counterpart. */
 int fdmla_device_error_flag(int reset);
 
+/* Sets that flag as a wait that gave up would (codes 41..44 and 51..53, else FDMLA_ERR_INVALID; synchronises): how a
+ * caller's handling of a time-out is tested without one.  No reference counterpart. */
+int fdmla_set_device_error_flag(int code);
+
 /*
  * Cache-latent DMLA forward.
  *   Q     [B, H, Sq, d_qk]

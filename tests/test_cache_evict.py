@@ -606,3 +606,43 @@ def test_reserved_rows_start_without_weight(cuda):
     assert c.evict([b], 100).tolist() == [list(range(100))]               # all weights equal: the lower rows stay
     c.reserve([b], 1)
     assert c.row_state(b)[1].tolist() == list(range(100)) + [130]
+
+
+# ------------------------------------------------------------------------------------------------ after a time-out
+def test_error_flag_takes_only_codes_of_waits():
+    from flashdmla import _lib
+    for code in (0, 4, 31, 40, 45, 50, 54, -1):
+        assert _lib.lib().fdmla_set_device_error_flag(code) == -1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens,H,Sq", [([500, 130, 7], 8, 33), ([300, 65], 16, 1)])
+def test_weights_stay_as_they_were_after_a_time_out(cuda, lens, H, Sq):
+    """While the flag of an earlier time-out stands a call adds nothing, not even what its scratch happened to hold; once it
+    is cleared, calls work again."""
+    import flashdmla as F
+    from flashdmla import _lib
+    L = _lib.lib()
+    inp = acc_inputs(lens, H, Sq, 576, 64, torch.bfloat16, True)
+    pool, table, phys, Q, weights, scale, m, l = inp
+    nbytes = L.fdmla_cache_accumulate_workspace_bytes(len(lens), H, Sq, 576, 64, table.shape[1], _lib.BF16)
+    assert (nbytes > 0) == (Sq > 1)                          # the window's query rows are split: partial sums in the scratch
+    dev = [t.to(cuda) for t in (Q, pool, table, torch.tensor(lens, dtype=torch.int32), m, l)]
+    w = weights.to(cuda)
+    ws = torch.full((max(nbytes // 4, 1),), 1.0, device=cuda)
+
+    def call():
+        ws.fill_(1.0)
+        rc = L.fdmla_cache_accumulate(*[t.data_ptr() for t in (*dev, w, ws)], nbytes, len(lens), H, Sq, 576, 64, table.shape[1],
+                                      pool.shape[0], scale, 1, _lib.BF16, torch.cuda.current_stream().cuda_stream)
+        assert rc == 0
+        torch.cuda.synchronize()
+    try:
+        assert L.fdmla_set_device_error_flag(52) == 0
+        call()
+        assert torch.equal(w.cpu(), weights)
+        assert F.device_error_flag(reset=True) == 52
+        call()
+    finally:
+        F.device_error_flag(reset=True)
+    check_accumulated(w.cpu(), inp, True)
