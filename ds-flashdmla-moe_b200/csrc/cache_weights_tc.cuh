@@ -43,6 +43,7 @@ struct TcShared {                                    // in front of the operands
     int dead, b0, tile0, n_tiles, scan[TC_THREADS / 32];
     alignas(16) float2 ml[2][QROWS];                 // m log2(e) and 1 / l of the tile's query rows
     int last[2][QROWS];                              // last key each of them sees
+    alignas(16) int left_out[2][4];                  // per epilogue warp: some of its rows see nothing (l <= 0)
 };
 
 struct TcProblem {
@@ -344,15 +345,24 @@ accumulate_kernel(const TcProblem p, const __grid_constant__ CUtensorMap tmQ, co
             }
         };
         // ... and keeps, in shared memory, m log2(e), 1 / l and the last key the row sees.  A row that sees nothing gets (inf, 0):
-        // every exponential is 0.
+        // every exponential of a finite score is 0.  Its scores need not be finite (a padded batch), so a tile with such a row is
+        // summed with the comparison that leaves terms out instead of multiplying them by 0.
         auto keep = [&](int buf, int n, int r0, const Stats &st) {
+            bool out = false;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const int c = L + 128 * i, r = r0 + c;
                 const bool seen = r < a.R && !(st.l[i] <= 0.f);
                 sh.ml[buf][c] = seen ? make_float2(st.m[i] * 1.4426950408889634f, 1.f / st.l[i]) : make_float2(CUDART_INF_F, 0.f);
                 sh.last[buf][c] = !seen ? -1 : (a.causal ? r % a.Sq + n - a.Sq : n - 1);
+                out |= r < a.R && !seen;
             }
+            out = __any_sync(0xffffffffu, out);
+            if (lane == 0) sh.left_out[buf][warp & 3] = out;
+        };
+        auto some_left_out = [&](int buf) {
+            const int4 o = *reinterpret_cast<const int4 *>(sh.left_out[buf]);
+            return (o.x | o.y | o.z | o.w) != 0;
         };
         // sum over the columns 0 .. cols - 1 of an accumulator
         auto sum_tile = [&](int acc, int buf, int cols, int t, bool masked) {
@@ -399,6 +409,7 @@ accumulate_kernel(const TcProblem p, const __grid_constant__ CUtensorMap tmQ, co
                 buf ^= 1;
                 keep(buf, n, 0, ml);
                 named_bar_sync(1, 128);
+                const bool some_out = some_left_out(buf);
                 for (int i = 0; i < w.count; ++i) {
                     const int acc = n_done & 1, t = w.t0 + i * KEYS + rank * 128 + L;
                     const long long row = t < n ? a.pg.row(b, t) : -1;           // under the tile's copies and MMAs
@@ -406,7 +417,7 @@ accumulate_kernel(const TcProblem p, const __grid_constant__ CUtensorMap tmQ, co
                     tc_fence_after_sync();
                     ++n_done;
                     float g = 0.f;
-                    if (ok) g = sum_tile(acc, buf, a.R, t, a.causal && w.t0 + (i + 1) * KEYS > n - a.Sq + 1);
+                    if (ok) g = sum_tile(acc, buf, a.R, t, some_out || (a.causal && w.t0 + (i + 1) * KEYS > n - a.Sq + 1));
                     release(acc);
                     if (ok) add(row, g);
                 }
@@ -429,7 +440,8 @@ accumulate_kernel(const TcProblem p, const __grid_constant__ CUtensorMap tmQ, co
                     ok = __all_sync(0xffffffffu, ok && mbar_wait(ACC_FULL(acc), (n_done >> 1) & 1));
                     tc_fence_after_sync();
                     ++n_done;
-                    if (ok) g += sum_tile(acc, buf, min(QROWS, a.R - r * QROWS), t, a.causal && w.t0 + KEYS > n - a.Sq + 1);
+                    if (ok) g += sum_tile(acc, buf, min(QROWS, a.R - r * QROWS), t,
+                                          some_left_out(buf) || (a.causal && w.t0 + KEYS > n - a.Sq + 1));
                     release(acc);
                 }
                 if (!ok || t >= n) continue;

@@ -608,6 +608,31 @@ def test_reserved_rows_start_without_weight(cuda):
     assert c.row_state(b)[1].tolist() == list(range(100)) + [130]
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens,H,Sq,d,page,dtype,causal", [
+    ([700, 64, 0], 16, 1, 576, 64, torch.bfloat16, True),     # the query rows of a step are resident
+    ([700, 64, 0], 64, 1, 576, 64, torch.bfloat16, True),
+    ([900, 300], 8, 5, 64, 64, torch.bfloat16, False),
+    ([1100, 500], 16, 40, 192, 64, torch.bfloat16, True),     # the query rows stream past
+    ([300, 40], 5, 3, 24, 16, torch.float32, True),           # CUDA cores
+])
+def test_query_rows_with_l_zero_add_nothing_whatever_they_hold(cuda, lens, H, Sq, d, page, dtype, causal):
+    """The rows of a padded batch: l = 0, and a query that is NaN, infinite, or large enough to overflow the score."""
+    import flashdmla as F
+    pool, table, phys, Q, weights, scale, m, l = acc_inputs(lens, H, Sq, d, page, dtype, causal)
+    dirty, m_dirty, l = Q.clone(), m.clone(), l.clone()
+    R = H * Sq
+    for b in range(len(lens)):
+        for r, v in ((0, float("nan")), (R // 2, float("inf")), (R - 1, 3e38)):
+            dirty[b].view(R, d)[r] = v
+            m_dirty[b].view(R)[r] = v
+            l[b].view(R)[r] = 0.0
+    w = weights.to(cuda)
+    F.accumulate_weights(*[t.to(cuda) for t in (dirty, pool, table, torch.tensor(lens, dtype=torch.int32), m_dirty, l)], w, scale, causal)
+    check_accumulated(w.cpu(), (pool, table, phys, Q, weights, scale, m, l), causal)
+    assert F.device_error_flag() == 0
+
+
 # ------------------------------------------------------------------------------------------------ after a time-out
 def test_error_flag_takes_only_codes_of_waits():
     from flashdmla import _lib
