@@ -213,10 +213,11 @@ accumulate_kernel(const TcProblem p, const __grid_constant__ CUtensorMap tmQ, co
         };
         Walker<ROWS> w(p, sh, unit);
         bool more = w.next(units);
-        while (ok && more) {
+        // Each lane waits for itself, so a wait that gives up may do so in some lanes only: they agree here, before the branch, since
+        // the lanes vote and exchange page ids inside.
+        while ((ok = __all_sync(0xffffffffu, ok)) && more) {
             Walker<ROWS> after = w;                    // the set behind this one: its resident operand is brought into L2 meanwhile
             more = after.next(units);
-            if (ROWS) ok = __all_sync(0xffffffffu, ok);
             if (visible(w) && ok) {
                 const int b = w.b;
                 int page = page_of(b, w.t0, w.n), r0 = 0, r1 = 0;

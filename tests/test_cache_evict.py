@@ -633,6 +633,44 @@ def test_query_rows_with_l_zero_add_nothing_whatever_they_hold(cuda, lens, H, Sq
     assert F.device_error_flag() == 0
 
 
+# lens, table rows beyond the longest sequence, H, Sq, d, causal: what a pair of CTAs (74 of them) has to do several times over.
+# Counts of tiles of 256 keys below are those of the lengths.
+MANY_TILES = [
+    ("resident queries, 294 tiles", [(97 * i) % 2501 for i in range(60)] + [0, 256, 257], 0, 16, 1, 64, True),
+    ("resident queries, masked", [(97 * i) % 2501 for i in range(60)], 0, 16, 4, 64, True),
+    ("resident queries, nine chunks, runs across sequences", [(331 * i) % 1801 for i in range(40)], 0, 32, 1, 576, True),
+    ("streamed queries, 3 splits of 5 row tiles", [(137 * i) % 1301 for i in range(30)], 0, 28, 40, 64, True),
+    ("streamed queries, not causal", [(137 * i) % 1301 for i in range(30)], 0, 28, 40, 64, False),
+    ("streamed queries, one split", [(97 * i) % 2501 for i in range(46)], 0, 10, 33, 64, True),
+    ("streamed queries, one split, not causal", [(97 * i) % 2501 for i in range(46)], 0, 10, 33, 64, False),
+    ("streamed queries, nine chunks, several row tiles an item", [(137 * i) % 1301 for i in range(34)], 0, 20, 41, 576, True),
+    ("streamed queries, row tiles that see nothing of an item", [(231 * i) % 1901 for i in range(30)], 0, 2, 700, 64, True),
+    ("streamed queries, a table far wider than the lengths", [700, 0, 260, 1], 16384, 24, 60, 128, True),
+    ("resident queries, a table far wider than the lengths", [700, 0, 260, 1], 16384, 64, 1, 128, True),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens,wider,H,Sq,d,causal", [c[1:] for c in MANY_TILES], ids=[c[0] for c in MANY_TILES])
+def test_accumulate_with_several_tiles_per_pair(cuda, lens, wider, H, Sq, d, causal):
+    """Reuse of the resident operand, of both accumulators and of the row statistics, runs that cross sequences, sums over
+    several tiles of query rows, with and without partial sums."""
+    import flashdmla as F
+    inp = acc_inputs(lens, H, Sq, d, 64, torch.bfloat16, causal)
+    pool, table, phys, Q, weights, scale, m, l = inp
+    wide = torch.full((len(lens), table.shape[1] + wider // 64), 10 ** 9, dtype=torch.int32)      # no page of the rest is looked at
+    for b, n in enumerate(lens):
+        wide[b, :(n + 63) // 64] = table[b, :(n + 63) // 64]
+    w = weights.to(cuda)
+    args = [t.to(cuda) for t in (Q, pool, wide, torch.tensor(lens, dtype=torch.int32), m, l)]
+    F.accumulate_weights(*args, w, scale, causal)
+    assert F.last_kernel() == "tcgen05" and F.device_error_flag() == 0
+    check_accumulated(w.cpu(), inp, causal)
+    w2 = weights.to(cuda)
+    F.accumulate_weights(*args, w2, scale, causal)
+    assert torch.equal(w, w2)
+
+
 # ------------------------------------------------------------------------------------------------ after a time-out
 def test_error_flag_takes_only_codes_of_waits():
     from flashdmla import _lib
