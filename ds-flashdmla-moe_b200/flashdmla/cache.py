@@ -153,6 +153,9 @@ class PagedLatentCache:
         """(page_table [n, max_pages], seqlens [n]) on the device for the listed sequences."""
         if not self.on_gpu:
             raise FlashDMLAError("device tables need a CUDA cache")
+        for s in slots:                          # an index out of range would be a device assert in the gather below
+            if not 0 <= s < self.max_seqs:
+                raise FlashDMLAError(f"there is no sequence slot {s}")
         idx = torch.tensor(list(slots), dtype=torch.long, device=self.device)
         return self.d_table.index_select(0, idx), self.d_len.index_select(0, idx)
 

@@ -98,6 +98,24 @@ def test_shrinking_gives_pages_back_without_a_gpu():
         c.evict([b], 2)                                                       # no CPU fallback
 
 
+def test_slots_outside_the_cache_are_refused_before_anything_is_launched():
+    """The tables are gathered on the GPU, where an index out of range would be a device assert.  Here the device side is the
+    host's own tensors."""
+    from flashdmla import FlashDMLAError
+    from flashdmla.cache import PagedLatentCache
+    c = PagedLatentCache(num_pages=10, page_size=4, d_qk=8, max_seqs=3, max_pages_per_seq=8, device="cpu", track_weights=True)
+    a = c.new_sequence()
+    c.reserve([a], 9)
+    c.on_gpu, c.d_table, c.d_len = True, c.h_table.clone(), c.h_len.clone()
+    assert c.tables([a, 2])[1].tolist() == [9, 0]
+    for slots in ([3], [-1], [a, 10 ** 6]):
+        for call in (lambda: c.tables(slots), lambda: c.evict(slots, 4), lambda: c.gather(slots, 1),
+                     lambda: c.decode(torch.zeros(len(slots), 2, 8), slots, 4)):
+            with pytest.raises(FlashDMLAError, match="slot"):
+                call()
+    assert c.length(a) == 9 and len(c.pages_of(a)) == 3
+
+
 def test_c_entry_points_refuse_bad_arguments():
     from flashdmla import _lib
     L = _lib.lib()
