@@ -471,6 +471,8 @@ def cache_stamp(weights, positions, page_table, start_pos, first_position, n_tok
     if weights.dtype != torch.float32 or positions.dtype != torch.int32 or weights.dim() != 2 or weights.shape != positions.shape \
             or not weights.is_contiguous() or not positions.is_contiguous():
         raise FlashDMLAError("weights (float32) and positions (int32) must be contiguous [num_pages, page_size] tensors")
+    if not 0 <= int(n_tokens) <= 2 ** 31 - 128:
+        raise FlashDMLAError("n_tokens must be between 0 and 2^31 - 128")
     num_pages, page_size = weights.shape
     page_table, start_pos, first_position = page_table.contiguous(), start_pos.contiguous(), first_position.contiguous()
     ctx, stream = _launch_on(weights)
@@ -526,8 +528,8 @@ def cache_evict(kv_pool, weights, positions, page_table, seqlens, next_position,
     _check_row_state(kv_pool, weights, positions)
     B, keep, recent = page_table.shape[0], int(keep), int(recent)
     _check_tables(page_table, B, seqlens, next_position)
-    if keep < 1 or not 0 <= recent <= keep:
-        raise FlashDMLAError("cache_evict needs keep >= 1 and 0 <= recent <= keep")
+    if not 1 <= keep <= 1 << 30 or not 0 <= recent <= keep:      # kept is allocated, and the binding cuts to 32 bits, below
+        raise FlashDMLAError("cache_evict needs 1 <= keep <= 2^30 and 0 <= recent <= keep")
     num_pages, page_size, d_qk = kv_pool.shape
     max_pages = page_table.shape[1]
     page_table, seqlens, next_position = page_table.contiguous(), seqlens.contiguous(), next_position.contiguous()

@@ -116,6 +116,21 @@ def test_slots_outside_the_cache_are_refused_before_anything_is_launched():
     assert c.length(a) == 9 and len(c.pages_of(a)) == 3
 
 
+def test_bounds_that_an_int_does_not_hold_are_refused(monkeypatch):
+    """Behind the binding they would be cut to 32 bits: keep = 2^32 + 5 would leave five rows."""
+    import flashdmla as F
+    from flashdmla import ops
+    monkeypatch.setattr(ops, "_need_cuda", lambda *t: None)                   # the checks of arguments alone, on CPU tensors
+    z = torch.zeros
+    state = (z(1, 4, 8), z(1, 4), z(1, 4).int())
+    for keep, recent in ((2 ** 32 + 5, 0), (2 ** 31, 0), (2 ** 30 + 1, 3), (0, 0), (4, 5)):
+        with pytest.raises(F.FlashDMLAError, match="keep"):
+            F.cache_evict(*state, z(1, 1).int(), z(1).int(), z(1).int(), keep, recent)
+    for n in (2 ** 32 + 1, 2 ** 31, -1):
+        with pytest.raises(F.FlashDMLAError, match="n_tokens"):
+            F.cache_stamp(*state[1:], z(1, 1).int(), z(1).int(), z(1).int(), n)
+
+
 def test_c_entry_points_refuse_bad_arguments():
     from flashdmla import _lib
     L = _lib.lib()
