@@ -115,6 +115,8 @@ class PagedLatentCache:
             want = (int(self.h_len[s]) + n_tokens + self.page_size - 1) // self.page_size
             if want > self.max_pages:
                 raise FlashDMLAError(f"sequence {s} would exceed max_pages_per_seq = {self.max_pages}")
+            if int(self.h_next[s]) + n_tokens > 2 ** 31 - 1:
+                raise FlashDMLAError(f"sequence {s} would pass position 2^31 - 1")
             need.append(max(0, want - have))
         if sum(need) > len(self._free_pages):
             raise FlashDMLAError(f"out of cache pages: need {sum(need)}, {len(self._free_pages)} free")

@@ -131,6 +131,20 @@ def test_bounds_that_an_int_does_not_hold_are_refused(monkeypatch):
             F.cache_stamp(*state[1:], z(1, 1).int(), z(1).int(), z(1).int(), n)
 
 
+def test_positions_that_an_int_does_not_hold_are_refused():
+    """A bounded cache may go on for ever, its positions are 32-bit."""
+    from flashdmla import FlashDMLAError
+    from flashdmla.cache import PagedLatentCache
+    c = PagedLatentCache(num_pages=10, page_size=4, d_qk=8, max_seqs=2, max_pages_per_seq=8, device="cpu", track_weights=True)
+    a, b = c.new_sequence(), c.new_sequence()
+    c.reserve([a], 3)
+    c.h_next[a] = 2 ** 31 - 3
+    assert c.reserve([a], 2).tolist() == [3] and c.position(a) == 2 ** 31 - 1
+    with pytest.raises(FlashDMLAError, match="position"):
+        c.reserve([b, a], 1)
+    assert c.position(a) == 2 ** 31 - 1 and c.length(a) == 5 and c.length(b) == 0 and c.free_pages == 8
+
+
 def test_c_entry_points_refuse_bad_arguments():
     from flashdmla import _lib
     L = _lib.lib()
