@@ -297,3 +297,54 @@ def test_random_shapes(cuda, seed):
     want, err = definition(x, Wg, ws, sh, k)
     out = F.moe_few(*[t.to(cuda) for t in (x, Wg, *ws)], k, tuple(t.to(cuda) for t in sh) if sh else None)
     check(out, want, err)
+
+
+# 2 to 16 tokens of wider layers: more than 256 * 148 elements of h, summed four columns a thread
+SMALL_BATCHES = [
+    # T, d, f, E, k, shared
+    (3, 1024, 2048, 9, 8, True),
+    (4, 256, 2048, 16, 8, True),
+    (5, 64, 4096, 8, 8, False),                               # one step of d: tiles are not cut
+    (16, 320, 1216, 24, 6, False),                            # half a tile of f at the end
+    (16, 192, 2496, 12, 4, True),
+    (9, 2112, 704, 11, 7, True),
+    (13, 512, 256, 20, 12, True),                             # more than nine terms in the weighted sum
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,d,f,E,k,shared", SMALL_BATCHES)
+def test_small_batches_of_wide_layers(cuda, T, d, f, E, k, shared):
+    import flashdmla as F
+    assert 1 < T <= 16 and T * (k + shared) * f > 256 * 148
+    x, Wg, ws, sh = weights(T, d, f, E, shared, torch.bfloat16, seed=T * 11 + E)
+    want, err = definition(x, Wg, ws, sh, k)
+    dev = [t.to(cuda) for t in (x, Wg, *ws)]
+    dsh = tuple(t.to(cuda) for t in sh) if sh else None
+    out = F.moe_few(*dev, k, dsh)
+    assert F.last_kernel() == "tcgen05" and F.device_error_flag() == 0
+    check(out, want, err)
+    for _ in range(3):
+        assert torch.equal(out, F.moe_few(*dev, k, dsh))
+    assert F.moe_few(*dev, k, dsh, out=dev[0]) is dev[0] and torch.equal(out, dev[0])        # in place of the tokens
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [1, 20])
+def test_outputs_stay_as_they_were_after_a_time_out(cuda, T):
+    """While the flag of an earlier time-out stands a call writes nothing; once it is cleared, calls work again."""
+    import flashdmla as F
+    from flashdmla import _lib
+    x, Wg, ws, sh = weights(T, 256, 128, 16, True, torch.bfloat16, 5)
+    want, err = definition(x, Wg, ws, sh, 4)
+    dev = [t.to(cuda) for t in (x, Wg, *ws)]
+    dsh = tuple(t.to(cuda) for t in sh)
+    out = torch.full((T, 256), 7.0, dtype=torch.bfloat16, device=cuda)
+    try:
+        assert _lib.lib().fdmla_set_device_error_flag(44) == 0
+        F.moe_few(*dev, 4, dsh, out=out)
+        assert (out == 7).all() and F.device_error_flag(reset=True) == 44
+        F.moe_few(*dev, 4, dsh, out=out)
+    finally:
+        F.device_error_flag(reset=True)
+    check(out, want, err)
