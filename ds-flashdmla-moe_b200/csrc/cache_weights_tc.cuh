@@ -20,8 +20,8 @@
 // Warp 0 issues the copies, warp 1 (of the leader) the MMAs, warps 2-5 read the accumulators.  Waits are bounded (codes 51-53).
 //
 // Measured, replayed from a CUDA graph with the copy of weights in front: 128 sequences of 4096 keys, 128 heads 108 us (604 MB of
-// rows at 6.6 TB/s inside the kernel); 32 queries of 128 heads over 5000 and 16384 keys 86 us (1.2 PFLOP/s, 67 % of the tensor
-// cycles; 320 to 340 cycles a chunk of 64 columns are latency of the 64 KB ring).
+// rows at 6.6 TB/s inside the kernel); 32 queries of 128 heads over 5000 and 16384 keys 86 us (1.2 PFLOP/s, 66 % of the tensor
+// cycles, 59 to 73 % by SM; a chunk of 64 columns takes 320 to 340 cycles where its MMAs need 256, with L2 at 18 % of its rate).
 #pragma once
 
 #include <atomic>
