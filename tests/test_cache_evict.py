@@ -244,6 +244,25 @@ def test_evict_matches_the_definition(cuda, lens, keep, recent, page, d, dtype, 
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("capacity", [9000, 131072, 700000])
+@pytest.mark.parametrize("kind", ["random", "ties", "wild"])
+def test_evict_with_a_table_far_wider_than_the_lengths(cuda, capacity, kind):
+    """The CTAs of a sequence share its rows by the table's capacity: some have none, and the others hold all of them."""
+    import flashdmla as F
+    lens, keep, recent, page, d = [700, 5000, 301, 64, 0, 300, 8999], 300, 40, 64, 64
+    case = evict_case(lens, keep, recent, page, d, torch.bfloat16, kind, seed=capacity)
+    pool, weights, positions, table, phys, nxt = case
+    wide = torch.full((len(lens), -(-capacity // page)), 10 ** 9, dtype=torch.int32)         # no page of the rest is looked at
+    for b, n in enumerate(lens):
+        wide[b, :-(-n // page)] = table[b, :-(-n // page)]
+    dp, dw, dpos = pool.to(cuda), weights.to(cuda), positions.to(cuda)
+    kept, new = F.cache_evict(dp, dw, dpos, wide.to(cuda), torch.tensor(lens, dtype=torch.int32, device=cuda),
+                              torch.tensor(nxt, dtype=torch.int32, device=cuda), keep, recent)
+    check_evicted((dp.cpu(), dw.cpu(), dpos.cpu(), kept.cpu(), new.cpu()), case, lens, keep, recent)
+    assert F.device_error_flag() == 0
+
+
+@pytest.mark.gpu
 def test_evict_in_a_graph_on_another_stream_with_shared_lengths(cuda):
     """Captured once, replayed on new contents; the new lengths overwrite the old ones (C entry point)."""
     import flashdmla as F
