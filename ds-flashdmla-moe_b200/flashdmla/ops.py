@@ -488,7 +488,7 @@ def accumulate_weights(Q, kv_pool, page_table, seqlens, m, l, weights, scale=Non
     Q [B,H,d_qk] (a decode step) or [B,H,Sq,d_qk] (a prompt, or its last Sq queries); m, l of the attention of the same
     queries over the same cache with the same scale, shaped like Q without its last dimension; weights
     [num_pages,page_size] fp32, changed in place and returned.  causal: query i sees keys t <= i + seqlens[b] - Sq.
-    Queries that see nothing (l = 0) add nothing; the sequences of one call should not share pages."""
+    Queries that see nothing, or are left out (l = 0), add nothing, whatever they hold; the sequences of one call should not share pages."""
     _need_cuda(Q, kv_pool, page_table, seqlens, m, l, weights)
     _same_dtype(Q, kv_pool)
     if Q.dim() not in (3, 4):

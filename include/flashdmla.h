@@ -425,7 +425,8 @@ int fdmla_cache_stamp(float *weights, int32_t *positions,
  * weights[row of key t of sequence b] += sum over query rows (h, i) that see t of exp(scale q_hi . k_t - m_hi) / l_hi.
  *   Q [B, H, Sq, d_qk] (Sq = 1: one decode step; Sq > 1: a prompt or its last Sq queries), m, l [B, H, Sq] fp32 as the
  *   attention of the same step returned them for the same scale; query i sees keys t <= i + seqlens[b] - Sq when causal,
- *   all seqlens[b] keys otherwise.  A query row with l <= 0 (nothing visible) gives nothing.
+ *   all seqlens[b] keys otherwise.  A query row with l <= 0 (nothing visible, or left out by the caller)
+ *   gives nothing, whatever its query and m hold.
  *   Sequences of one call should own their pages; if two share one, its weights receive both sums (in either order).
  *   workspace: fdmla_cache_accumulate_workspace_bytes() bytes of device scratch, 256-byte aligned (may be 0 bytes: NULL).
  *   bf16 with d_qk a multiple of 64 up to 576 and page_size a multiple of 64 runs on the tensor cores, everything else with
